@@ -317,6 +317,81 @@ int lastro_batch_set_options(lastro_batch *batch, int32_t use_graphs, int32_t us
 int lastro_batch_set_wait_limit(lastro_batch *batch, uint64_t wait_ns);
 void lastro_batch_destroy(lastro_batch *batch);
 
+/* ---- 8-bit KV cache: append, attention, eviction (no counterpart in the reference, whose cache is f32 and only grows) --
+ * A paged cache of one layer that holds K and V in one byte a value, for contexts longer than a bf16 cache has room for
+ * and for contexts held to a budget.  The caller owns every buffer, all of them device memory; a call enqueues its
+ * kernels on the context's stream and returns without allocating or synchronising, so it may be captured into a graph.
+ *   pages of 64 slots, blocks of 16 slots; codes [num_pages, kv_heads, 64, head_dim] bytes, e4m3 or int8 (16-byte
+ *   aligned); scales [num_pages, kv_heads, 4] f32, one per block and KV head, powers of two (16-byte aligned); the value
+ *   held is code * scale.  Slot s of sequence b is row s % 64 of page page_table[b * max_pages + s / 64].
+ * Quantisation of a block: scale = the smallest power of two 2^e, e >= -126, with max |value| <= qmax * 2^e (qmax 448 for
+ * e4m3, 127 for int8), codes = the nearest representable value / scale, ties to even.  A power of two makes the division
+ * exact, so a code moved to another scale is rounded once, and not at all when the scale shrinks.  A block that is given
+ * a value that is not finite gets a NaN scale: all of it reads as NaN.  (Magnitudes above 3.2e38 may round to infinity.)
+ * Sequence lengths and row offsets are read on the device.  What the host cannot check there is checked by the kernels:
+ * a page number outside the pool, a length outside the page table, row offsets outside the rows or beyond max_new make
+ * the kernel skip that page or sequence and leave a LASTRO_KV8_BAD_* code in *status (device memory, may be NULL; never
+ * cleared by the library).  Calls that share a cache, a workspace or outputs must not overlap on the GPU. */
+#define LASTRO_KV8_E4M3 1
+#define LASTRO_KV8_INT8 2
+#define LASTRO_KV8_PAGE 64
+#define LASTRO_KV8_BLOCK 16
+#define LASTRO_KV8_BAD_PAGE 1    /* page number outside [0, num_pages): its slots are skipped */
+#define LASTRO_KV8_BAD_LENGTH 2  /* length below 0 or beyond the page table, queries or mass row: the sequence is skipped */
+#define LASTRO_KV8_BAD_OFFSET 3  /* row offsets that descend, pass max_new or leave the rows: the sequence is skipped */
+typedef struct {
+    int32_t format;                     /* LASTRO_KV8_E4M3 or LASTRO_KV8_INT8 */
+    int32_t n_seqs, kv_heads, head_dim; /* head_dim 64 or 128 */
+    int32_t num_pages, max_pages;       /* pages in the pool; page table entries of one sequence */
+    void *k, *v;
+    float *k_scale, *v_scale;
+    const int32_t *page_table; /* [n_seqs, max_pages]; entries past a sequence's pages are not read */
+    int32_t *status;           /* one word or NULL */
+} lastro_kv8;
+/* activation rows [rows, heads, head_dim]: element (r, h, j) at ptr[r * row_stride + h * head_stride + j] (strides in
+ * elements, any order); dtype LASTRO_DTYPE_BF16 or LASTRO_DTYPE_F32 */
+typedef struct {
+    void *ptr;
+    int32_t dtype, rows;
+    int64_t row_stride, head_stride;
+} lastro_rows;
+/* quantises new K and V rows into the cache: rows [new_off[b], new_off[b + 1]) (device, n_seqs + 1 offsets; at most
+ * max_new rows a sequence) go to slots lens[b].. of sequence b, whose pages the page table already names.  A block that
+ * holds earlier rows keeps its scale when the new ones fit it, else takes the larger scale and its codes are rounded to it.
+ * Slots past the last row keep what they hold.  lens_out[b] = the new length (must not overlap lens); mass, when not
+ * NULL, is the accumulated-weight array [n_seqs, kv_heads, mass_stride], whose new slots start at 0. */
+int lastro_kv8_append(lastro_ctx *ctx, const lastro_kv8 *kv, const int32_t *lens, const int32_t *new_off,
+                      int32_t max_new, const lastro_rows *k, const lastro_rows *v, int32_t *lens_out, float *mass,
+                      int64_t mass_stride);
+/* bytes of workspace lastro_kv8_attend needs for `heads` query heads and at most max_new queries a sequence */
+int lastro_kv8_attend_workspace(lastro_ctx *ctx, const lastro_kv8 *kv, int32_t heads, int32_t max_new,
+                                int32_t with_mass, size_t *bytes);
+/* grouped-query attention over the cache: rows [q_off[b], q_off[b + 1]) of q (heads a multiple of kv_heads) are the last
+ * queries of sequence b, whose length lens[b] counts their own slots: query i of n sees slots [0, lens[b] - n + i].
+ * out = softmax(scale * q k) v in q's dtype; a query that sees no slot gets zeros, one that holds a value that is not
+ * finite gets NaN.  mass_out, when not NULL: [n_seqs, kv_heads, mass_stride] with mass_out[b, h, t] = mass_in[b, h, t] (0
+ * when mass_in is NULL) + the attention weights slot t received from every query and every head of group h, for
+ * t < lens[b]; other entries are not written; mass_in may be mass_out.  Products accumulate in f32; bf16 rows are exact
+ * operands and their weights are rounded to f16 (11 bits, below the output's 8), f32 rows and weights are carried as two
+ * f16 terms (22 bits).  The same call on the same data gives the same bits. */
+int lastro_kv8_attend(lastro_ctx *ctx, const lastro_kv8 *kv, const int32_t *lens, const int32_t *q_off, int32_t max_new,
+                      int32_t heads, const lastro_rows *q, float scale, const lastro_rows *out, const float *mass_in,
+                      float *mass_out, int64_t mass_stride, void *workspace, size_t workspace_bytes);
+/* eviction by accumulated weight: a sequence longer than `budget` keeps, per KV head, its last `recent` slots and of the
+ * slots before them the budget - recent with the largest mass (ties: the lowest slot; NaN counts as the largest), in
+ * their order; a shorter one keeps all.  The kept rows are written densely to dst (the same format, heads, head_dim and
+ * n_seqs; other pages than any of src's sequences use), each block quantised anew from the values src held.
+ * kept [n_seqs, kv_heads, budget] receives the kept slots, -1 past the last; mass_out (may be NULL) [n_seqs, kv_heads,
+ * mass_out_stride] their mass (nothing past the last is written); lens_out [n_seqs] the new lengths.  mass may be NULL
+ * when recent == budget. */
+int lastro_kv8_evict(lastro_ctx *ctx, const lastro_kv8 *src, const lastro_kv8 *dst, const int32_t *lens, int32_t budget,
+                     int32_t recent, const float *mass, int64_t mass_stride, int32_t *kept, int32_t *lens_out,
+                     float *mass_out, int64_t mass_out_stride);
+/* the values of slots [pos0[b], pos0[b] + n) of every sequence: k_out / v_out [n_seqs, n, kv_heads, head_dim] (either may
+ * be NULL; 16-byte aligned), bf16 (exact: a code has at most 8 significant bits) or f32; zeros at and past lens[b] */
+int lastro_kv8_read(lastro_ctx *ctx, const lastro_kv8 *kv, const int32_t *lens, const int32_t *pos0, int32_t n,
+                    void *k_out, void *v_out, int32_t dtype);
+
 /* ---- text I/O: byte-level BPE tokenizer and the Granite 3.1 chat template (rust/moe-rt/src/tokenizador.rs) ----
  * Host-only.  Replaces Tokenizador (tokenizador.rs:192-467), renderiza_chat (:512-541) and formata_data (:544-561).
  * Errors: LASTRO_E_ARG for bad arguments, text that is not UTF-8, an id outside the vocabulary, or an output buffer

@@ -1,0 +1,60 @@
+// 8-bit KV cache: kernel arguments and launchers (kernels in kv8.cu, C ABI in kv8_capi.cu).
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "../../include/lastro_b200.h"
+
+namespace lastro {
+
+constexpr int kKv8Page = LASTRO_KV8_PAGE, kKv8Block = LASTRO_KV8_BLOCK;
+constexpr int kKv8Blocks = kKv8Page / kKv8Block;  // blocks (scales) of one page and head
+
+struct Kv8AppendArgs {
+    lastro_kv8 kv;
+    const int32_t *lens, *new_off;
+    lastro_rows k, v;
+    int32_t max_new, blocks;  // blocks: most blocks one sequence's new rows touch
+    int32_t* lens_out;
+    float* mass;
+    int64_t mass_stride;
+};
+
+struct Kv8AttendArgs {
+    lastro_kv8 kv;
+    const int32_t *lens, *q_off;
+    lastro_rows q, out;
+    int32_t max_new, heads, group;
+    float scale;
+    const float* mass_in;
+    float* mass_out;
+    int64_t mass_stride;
+    float* lse;  // [rows, heads]: log of each softmax's sum, what the weights are rebuilt from
+};
+
+struct Kv8EvictArgs {
+    lastro_kv8 src, dst;
+    const int32_t* lens;
+    int32_t budget, recent;
+    const float* mass;
+    int64_t mass_stride;
+    int32_t *kept, *lens_out;
+    float* mass_out;
+    int64_t mass_out_stride;
+};
+
+struct Kv8ReadArgs {
+    lastro_kv8 kv;
+    const int32_t *lens, *pos0;
+    int32_t n;
+    void *k_out, *v_out;
+    int32_t f32;
+};
+
+cudaError_t launch_kv8_append(const Kv8AppendArgs& a, cudaStream_t s);
+cudaError_t launch_kv8_attend(const Kv8AttendArgs& a, cudaStream_t s);
+cudaError_t launch_kv8_evict(const Kv8EvictArgs& a, cudaStream_t s);
+cudaError_t launch_kv8_read(const Kv8ReadArgs& a, cudaStream_t s);
+
+}  // namespace lastro

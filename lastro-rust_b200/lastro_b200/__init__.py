@@ -23,6 +23,10 @@ HEADER = os.path.join(PKG_DIR, "..", "include", "lastro_b200.h")
 OK, E_ARG, E_CUDA, E_POISONED, E_FULL, E_NOMEM, E_UNSUPPORTED, E_STATE, E_IO = range(9)
 TRACE_WORDS = 11  # LASTRO_TRACE_WORDS: start, release, exit, 8 milestones per CTA
 DTYPE_BF16, DTYPE_F32, DTYPE_Q8_0 = 1, 2, 3
+LEGACY_STREAM = 1  # cudaStreamLegacy: a Context on the default stream (0 and None make a stream of the context's own)
+KV8_FORMATS = {"e4m3": 1, "int8": 2}
+KV8_PAGE, KV8_BLOCK = 64, 16
+KV8_BAD_PAGE, KV8_BAD_LENGTH, KV8_BAD_OFFSET = 1, 2, 3
 
 _lib = None
 
@@ -46,6 +50,18 @@ class ModelDesc(C.Structure):
                [(n, C.c_float) for n in ("rope_theta", "eps", "embedding_multiplier", "residual_multiplier",
                                          "attention_multiplier", "logits_scaling")] + \
                [("weight_dtype", C.c_int32), ("kv_dtype", C.c_int32)]
+
+
+class Kv8Desc(C.Structure):
+    """lastro_kv8"""
+    _fields_ = [(n, C.c_int32) for n in ("format", "n_seqs", "kv_heads", "head_dim", "num_pages", "max_pages")] + \
+               [(n, C.c_void_p) for n in ("k", "v", "k_scale", "v_scale", "page_table", "status")]
+
+
+class Rows(C.Structure):
+    """lastro_rows: activation rows [rows, heads, head_dim] on the device, strides in elements."""
+    _fields_ = [("ptr", C.c_void_p), ("dtype", C.c_int32), ("rows", C.c_int32), ("row_stride", C.c_int64),
+                ("head_stride", C.c_int64)]
 
 
 EXPORTS = {
@@ -130,6 +146,17 @@ EXPORTS = {
                                      C.c_void_p, C.c_int32, C.c_void_p]),
     "lastro_batch_trace_raw": (C.c_int, [C.c_void_p, C.c_int32, C.c_void_p, C.c_int32]),
     "lastro_batch_destroy": (None, [C.c_void_p]),
+    "lastro_kv8_append": (C.c_int, [C.c_void_p, C.POINTER(Kv8Desc), C.c_void_p, C.c_void_p, C.c_int32, C.POINTER(Rows),
+                                    C.POINTER(Rows), C.c_void_p, C.c_void_p, C.c_int64]),
+    "lastro_kv8_attend_workspace": (C.c_int, [C.c_void_p, C.POINTER(Kv8Desc), C.c_int32, C.c_int32, C.c_int32,
+                                              C.POINTER(C.c_size_t)]),
+    "lastro_kv8_attend": (C.c_int, [C.c_void_p, C.POINTER(Kv8Desc), C.c_void_p, C.c_void_p, C.c_int32, C.c_int32,
+                                    C.POINTER(Rows), C.c_float, C.POINTER(Rows), C.c_void_p, C.c_void_p, C.c_int64,
+                                    C.c_void_p, C.c_size_t]),
+    "lastro_kv8_evict": (C.c_int, [C.c_void_p, C.POINTER(Kv8Desc), C.POINTER(Kv8Desc), C.c_void_p, C.c_int32, C.c_int32,
+                                   C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64]),
+    "lastro_kv8_read": (C.c_int, [C.c_void_p, C.POINTER(Kv8Desc), C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p,
+                                  C.c_void_p, C.c_int32]),
 }
 
 HANDLE_BYTES = 64  # cudaIpcMemHandle_t
@@ -768,3 +795,74 @@ class GpuBatch:
         # at interpreter exit (module globals already cleared) the process's CUDA context goes with the process
         if getattr(self, "h", None) and not _finalizing():
             self.close()
+
+
+_ROW_DTYPES = {"torch.bfloat16": DTYPE_BF16, "torch.float32": DTYPE_F32, "bf16": DTYPE_BF16, "f32": DTYPE_F32}
+
+
+def _dev(x):
+    """A device address: an int, None, or anything with data_ptr() (a torch tensor)."""
+    return x if x is None or isinstance(x, int) else x.data_ptr()
+
+
+def rows_of(t) -> Rows:
+    """The lastro_rows of a torch-like device tensor [rows, heads, head_dim], bf16 or f32, the last axis dense."""
+    rows, head = t.stride()[:2]
+    dtype = _ROW_DTYPES.get(str(t.dtype))
+    if dtype is None or t.ndim != 3 or t.stride(2) != 1:
+        raise LastroError(E_ARG, f"rows: {tuple(t.shape)} {t.dtype} with strides {t.stride()} (bf16 or f32, last axis dense)")
+    return Rows(t.data_ptr(), dtype, t.shape[0], rows, head)
+
+
+class Kv8Cache:
+    """One layer's paged KV cache in 8 bits (lastro_kv8): append, attend, evict, read.
+
+    The caller owns the device buffers (addresses as ints, or torch tensors): k, v codes [num_pages, kv_heads, 64,
+    head_dim] bytes, k_scale, v_scale [num_pages, kv_heads, 4] f32, page_table [n_seqs, max_pages] int32, status one int32
+    word or None (a KV8_BAD_* code when a kernel met a page, length or offset it could not use).  Arguments named lens,
+    new_off, q_off, pos0, lens_out and kept are int32 on the device, mass arrays f32.  Every call enqueues on the
+    context's stream and returns; tensors passed in are not kept alive by it."""
+
+    def __init__(self, ctx: Context, fmt: str, n_seqs: int, kv_heads: int, head_dim: int, num_pages: int, max_pages: int,
+                 k, v, k_scale, v_scale, page_table, status=None):
+        if fmt not in KV8_FORMATS:
+            raise LastroError(E_ARG, f"format {fmt!r} (one of {', '.join(KV8_FORMATS)})")
+        self.ctx = ctx
+        self.buffers = (k, v, k_scale, v_scale, page_table, status)  # tensors live as long as the cache
+        self.desc = Kv8Desc(KV8_FORMATS[fmt], n_seqs, kv_heads, head_dim, num_pages, max_pages,
+                            *(_dev(x) for x in self.buffers))
+
+    def append(self, lens, new_off, max_new: int, k: Rows, v: Rows, lens_out, mass=None, mass_stride: int = 0):
+        """Quantise rows [new_off[b], new_off[b + 1]) of k and v into slots lens[b].. of each sequence
+        (lastro_kv8_append)."""
+        self.ctx.check(lib().lastro_kv8_append(self.ctx.h, self.desc, _dev(lens), _dev(new_off), max_new, k, v,
+                                               _dev(lens_out), _dev(mass), mass_stride))
+
+    def attend_workspace(self, heads: int, max_new: int, with_mass: bool) -> int:
+        """Bytes of workspace attend() needs."""
+        n = C.c_size_t()
+        self.ctx.check(lib().lastro_kv8_attend_workspace(self.ctx.h, self.desc, heads, max_new, int(with_mass),
+                                                         C.byref(n)))
+        return n.value
+
+    def attend(self, lens, q_off, max_new: int, heads: int, q: Rows, scale: float, out: Rows, workspace,
+               workspace_bytes: int, mass_in=None, mass_out=None, mass_stride: int = 0):
+        """out = softmax(scale * q k) v over the slots each query sees; mass_out = mass_in + the weights each slot
+        received (lastro_kv8_attend)."""
+        self.ctx.check(lib().lastro_kv8_attend(self.ctx.h, self.desc, _dev(lens), _dev(q_off), max_new, heads, q, scale,
+                                               out, _dev(mass_in), _dev(mass_out), mass_stride, _dev(workspace),
+                                               workspace_bytes))
+
+    def evict(self, dst: "Kv8Cache", lens, budget: int, recent: int, mass, mass_stride: int, kept, lens_out,
+              mass_out=None, mass_out_stride: int = 0):
+        """Cut every sequence to `budget` slots by accumulated mass, its kept rows written to dst's pages
+        (lastro_kv8_evict)."""
+        self.ctx.check(lib().lastro_kv8_evict(self.ctx.h, self.desc, dst.desc, _dev(lens), budget, recent, _dev(mass),
+                                              mass_stride, _dev(kept), _dev(lens_out), _dev(mass_out), mass_out_stride))
+
+    def read(self, lens, pos0, n: int, k_out, v_out, dtype: str):
+        """The values of slots [pos0[b], pos0[b] + n) of every sequence as bf16 or f32 (lastro_kv8_read)."""
+        if dtype not in ("bf16", "f32"):
+            raise LastroError(E_ARG, f"dtype {dtype!r} (bf16 or f32)")
+        self.ctx.check(lib().lastro_kv8_read(self.ctx.h, self.desc, _dev(lens), _dev(pos0), n, _dev(k_out), _dev(v_out),
+                                             _ROW_DTYPES[dtype]))
