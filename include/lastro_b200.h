@@ -339,6 +339,7 @@ void lastro_batch_destroy(lastro_batch *batch);
 #define LASTRO_KV8_BAD_PAGE 1    /* page number outside [0, num_pages): its slots are skipped */
 #define LASTRO_KV8_BAD_LENGTH 2  /* length below 0 or beyond the page table, queries or mass row: the sequence is skipped */
 #define LASTRO_KV8_BAD_OFFSET 3  /* row offsets that descend, pass max_new or leave the rows: the sequence is skipped */
+#define LASTRO_KV8_BAD_WAIT 4    /* a copy inside a kernel did not arrive within its bound: outputs are not valid */
 typedef struct {
     int32_t format;                     /* LASTRO_KV8_E4M3 or LASTRO_KV8_INT8 */
     int32_t n_seqs, kv_heads, head_dim; /* head_dim 64 or 128 */

@@ -1,113 +1,11 @@
-// 8-bit KV cache: append (quantise), attention, eviction, read-back.  Layout and rules in include/lastro_b200.h.
-#include <cuda_fp8.h>
+// 8-bit KV cache: append (quantise), eviction, read-back (attention in kv8_attend.cu).  Layout and rules in
+// include/lastro_b200.h.
 #include <cuda_runtime.h>
 
-#include "common.cuh"
-#include "kv8.h"
+#include "kv8.cuh"
 
 namespace lastro {
 namespace {
-
-constexpr int E4M3 = LASTRO_KV8_E4M3, INT8 = LASTRO_KV8_INT8;
-
-// ---- checks on device data ------------------------------------------------------------------------------------------
-LDEV void report(const lastro_kv8& kv, int code) {
-    if (kv.status) atomicExch(kv.status, code);
-}
-
-// the page of slot `slot` of sequence b, or -1
-LDEV int page_of(const lastro_kv8& kv, int b, int slot) {
-    const int p = __ldg(kv.page_table + (int64_t)b * kv.max_pages + slot / kKv8Page);
-    if ((unsigned)p < (unsigned)kv.num_pages) return p;
-    report(kv, LASTRO_KV8_BAD_PAGE);
-    return -1;
-}
-
-// a sequence's length, 0 when it is not one the page table (or `most` slots) can hold
-LDEV int seq_len(const lastro_kv8& kv, const int32_t* lens, int b, int64_t most) {
-    const int n = __ldg(lens + b);
-    if (n >= 0 && n <= most) return n;
-    report(kv, LASTRO_KV8_BAD_LENGTH);
-    return 0;
-}
-
-// rows of sequence b: first row, and their number (0 when the offsets are not usable)
-LDEV int seq_rows(const lastro_kv8& kv, const int32_t* off, int b, int rows, int max_new, int& first) {
-    first = __ldg(off + b);
-    const int end = __ldg(off + b + 1);
-    if (first >= 0 && end >= first && end <= rows && end - first <= max_new) return end - first;
-    report(kv, LASTRO_KV8_BAD_OFFSET);
-    return 0;
-}
-
-// ---- values, codes, scales ------------------------------------------------------------------------------------------
-// The scale of a block whose largest magnitude has the bits `amax` (sign cleared; NaN and infinities order above every
-// finite value): with amax = 1.f * 2^E it is 2^(E-8) or 2^(E-7) for e4m3 (448 = 1.75 * 2^8), 2^(E-6) or 2^(E-5) for int8
-// (127 = 1.984375 * 2^6).
-template <int FMT>
-LDEV float scale_for(uint32_t amax) {
-    if (amax >= 0x7f800000u) return __uint_as_float(0x7fc00000u);
-    const uint32_t top = FMT == E4M3 ? 0x600000u : 0x7e0000u;
-    const int e = (int)(amax >> 23) - (FMT == E4M3 ? 8 : 6) + ((amax & 0x7fffffu) > top);
-    return __uint_as_float((uint32_t)max(e, 1) << 23);
-}
-
-// 1 / s of a power of two s = 2^e, -126 <= e <= 122: exact
-LDEV float inverse(float s) { return __uint_as_float((254u << 23) - (__float_as_uint(s) & 0x7f800000u)); }
-
-template <int FMT>
-LDEV uint32_t encode4(float a, float b, float c, float d) {
-    if (FMT == E4M3) {
-        const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
-        const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
-        return lo | (hi << 16);
-    }
-    return (uint32_t)(__float2int_rn(a) & 0xff) | (uint32_t)(__float2int_rn(b) & 0xff) << 8 |
-           (uint32_t)(__float2int_rn(c) & 0xff) << 16 | (uint32_t)(__float2int_rn(d) & 0xff) << 24;
-}
-
-template <int FMT>
-LDEV void decode4(uint32_t w, float (&v)[4]) {
-    if (FMT == E4M3) {
-        const float2 lo = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w & 0xffff), __NV_E4M3)));
-        const float2 hi = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w >> 16), __NV_E4M3)));
-        v[0] = lo.x, v[1] = lo.y, v[2] = hi.x, v[3] = hi.y;
-    } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = (float)(int8_t)(w >> (8 * i));
-    }
-}
-
-// 8 consecutive values of an activation row; `vec`: every such group is 16-byte aligned
-LDEV void load8(const lastro_rows& r, int64_t at, bool vec, float (&v)[8]) {
-    if (r.dtype == LASTRO_DTYPE_F32) {
-        const float* p = static_cast<const float*>(r.ptr) + at;
-        if (vec) {
-            const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
-            v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = __ldg(p + i);
-        }
-    } else {
-        const uint16_t* p = static_cast<const uint16_t*>(r.ptr) + at;
-        if (vec) {
-            const uint4 a = __ldg(reinterpret_cast<const uint4*>(p));
-            v[0] = bf_lo(a.x), v[1] = bf_hi(a.x), v[2] = bf_lo(a.y), v[3] = bf_hi(a.y);
-            v[4] = bf_lo(a.z), v[5] = bf_hi(a.z), v[6] = bf_lo(a.w), v[7] = bf_hi(a.w);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = __uint_as_float((uint32_t)__ldg(p + i) << 16);
-        }
-    }
-}
-
-LDEV bool vec_rows(const lastro_rows& r) {
-    const int64_t e = r.dtype == LASTRO_DTYPE_F32 ? 4 : 2;
-    return ((reinterpret_cast<uintptr_t>(r.ptr) | (uintptr_t)(r.row_stride * e) | (uintptr_t)(r.head_stride * e)) & 15) == 0;
-}
-
-LDEV uint32_t warp_umax(uint32_t v) { return __reduce_max_sync(0xffffffffu, v); }
 
 // ---- append ---------------------------------------------------------------------------------------------------------
 // One warp quantises one block (16 slots) of K or V of one head: its new rows pass through registers once (a lane holds
@@ -233,103 +131,6 @@ __global__ void __launch_bounds__(256) kv8_read_kernel(const __grid_constant__ K
                 reinterpret_cast<uint4*>(out)[i] = o;
             }
         }
-    }
-}
-
-// ---- attention ------------------------------------------------------------------------------------------------------
-// One warp per query row and head walks the sequence's visible slots with a running maximum and sum.
-template <int FMT, int D>
-LDEV void head_slice(const void* codes, int64_t row, int lane, float s, float (&v)[D / 32]) {
-    constexpr int V = D / 32;
-    const uint8_t* p = static_cast<const uint8_t*>(codes) + row * D + lane * V;
-    float t[4];
-    decode4<FMT>(V == 4 ? __ldg(reinterpret_cast<const uint32_t*>(p)) : (uint32_t)__ldg(reinterpret_cast<const uint16_t*>(p)), t);
-#pragma unroll
-    for (int i = 0; i < V; ++i) v[i] = t[i] * s;
-}
-
-LDEV float row_value(const lastro_rows& r, int64_t at) {
-    return r.dtype == LASTRO_DTYPE_F32 ? __ldg(static_cast<const float*>(r.ptr) + at)
-                                       : __uint_as_float((uint32_t)__ldg(static_cast<const uint16_t*>(r.ptr) + at) << 16);
-}
-
-LDEV void store_value(const lastro_rows& r, int64_t at, float v) {
-    if (r.dtype == LASTRO_DTYPE_F32)
-        static_cast<float*>(r.ptr)[at] = v;
-    else
-        static_cast<uint16_t*>(r.ptr)[at] = f32_to_bf16_rne(v);
-}
-
-template <int FMT, int D>
-__global__ void __launch_bounds__(256) kv8_attend_kernel(const __grid_constant__ Kv8AttendArgs a) {
-    constexpr int V = D / 32;
-    const int lane = threadIdx.x & 31, b = blockIdx.y;
-    int64_t most = (int64_t)a.kv.max_pages * kKv8Page;
-    if (a.mass_out) most = min(most, a.mass_stride);
-    const int len = seq_len(a.kv, a.lens, b, most);
-    int first;
-    const int n = seq_rows(a.kv, a.q_off, b, a.q.rows, a.max_new, first);
-    for (int64_t u = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); u < (int64_t)n * a.heads; u += (int64_t)gridDim.x * 8) {
-        const int i = (int)(u / a.heads), hq = (int)(u % a.heads), h = hq / a.group;
-        float q[V], o[V] = {}, m = -INFINITY, l = 0.0f;
-#pragma unroll
-        for (int e = 0; e < V; ++e)
-            q[e] = row_value(a.q, (int64_t)(first + i) * a.q.row_stride + hq * a.q.head_stride + lane * V + e) * a.scale;
-        for (int t = 0; t < len - n + i + 1; ++t) {
-            const int page = page_of(a.kv, b, t);
-            if (page < 0) continue;
-            const int64_t tile = (int64_t)page * a.kv.kv_heads + h;
-            const int64_t row = tile * kKv8Page + t % kKv8Page, blk = tile * kKv8Blocks + t % kKv8Page / kKv8Block;
-            float k[V], v[V], s = 0.0f;
-            head_slice<FMT, D>(a.kv.k, row, lane, __ldg(a.kv.k_scale + blk), k);
-            head_slice<FMT, D>(a.kv.v, row, lane, __ldg(a.kv.v_scale + blk), v);
-#pragma unroll
-            for (int e = 0; e < V; ++e) s = fmaf(q[e], k[e], s);
-            s = warp_sum(s);
-            const float mn = s > m || s != s ? s : m, c = m == -INFINITY ? 0.0f : expf(m - mn), p = expf(s - mn);
-            l = l * c + p;
-#pragma unroll
-            for (int e = 0; e < V; ++e) o[e] = fmaf(p, v[e], o[e] * c);
-            m = mn;
-        }
-#pragma unroll
-        for (int e = 0; e < V; ++e)
-            store_value(a.out, (int64_t)(first + i) * a.out.row_stride + hq * a.out.head_stride + lane * V + e,
-                        l == 0.0f ? 0.0f : o[e] / l);
-        if (lane == 0) a.lse[(int64_t)(first + i) * a.heads + hq] = m + logf(l);
-    }
-}
-
-// the weights each slot received, rebuilt from the scores and the softmax sums: one warp per slot and KV head
-template <int FMT, int D>
-__global__ void __launch_bounds__(256) kv8_mass_kernel(const __grid_constant__ Kv8AttendArgs a) {
-    constexpr int V = D / 32;
-    const int lane = threadIdx.x & 31, b = blockIdx.y, H = a.kv.kv_heads;
-    const int len = seq_len(a.kv, a.lens, b, min((int64_t)a.kv.max_pages * kKv8Page, a.mass_stride));
-    int first;
-    const int n = seq_rows(a.kv, a.q_off, b, a.q.rows, a.max_new, first);
-    for (int64_t u = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); u < (int64_t)len * H; u += (int64_t)gridDim.x * 8) {
-        const int t = (int)(u / H), h = (int)(u % H);
-        const int page = page_of(a.kv, b, t);
-        float sum = 0.0f;
-        if (page >= 0) {
-            const int64_t tile = (int64_t)page * H + h;
-            float k[V];
-            head_slice<FMT, D>(a.kv.k, tile * kKv8Page + t % kKv8Page, lane,
-                               __ldg(a.kv.k_scale + tile * kKv8Blocks + t % kKv8Page / kKv8Block), k);
-            for (int i = max(0, t - (len - n)); i < n; ++i)
-                for (int g = 0; g < a.group; ++g) {
-                    const int hq = h * a.group + g;
-                    float s = 0.0f;
-#pragma unroll
-                    for (int e = 0; e < V; ++e)
-                        s = fmaf(row_value(a.q, (int64_t)(first + i) * a.q.row_stride + hq * a.q.head_stride + lane * V + e) *
-                                     a.scale, k[e], s);
-                    sum += expf(warp_sum(s) - a.lse[(int64_t)(first + i) * a.heads + hq]);
-                }
-        }
-        const int64_t at = ((int64_t)b * H + h) * a.mass_stride + t;
-        if (lane == 0) a.mass_out[at] = (a.mass_in ? a.mass_in[at] : 0.0f) + sum;
     }
 }
 
@@ -509,12 +310,6 @@ __global__ void __launch_bounds__(256) kv8_gather_kernel(const __grid_constant__
 }
 
 // ---- variants -------------------------------------------------------------------------------------------------------
-template <typename F>
-cudaError_t by_shape(const lastro_kv8& kv, F f) {
-    if (kv.format == E4M3) return kv.head_dim == 64 ? f.template run<E4M3, 64>() : f.template run<E4M3, 128>();
-    return kv.head_dim == 64 ? f.template run<INT8, 64>() : f.template run<INT8, 128>();
-}
-
 unsigned int blocks_of(int64_t units, int per) { return (unsigned int)((units + per - 1) / per); }
 
 struct AppendLaunch {
@@ -524,21 +319,6 @@ struct AppendLaunch {
     cudaError_t run() {
         const int64_t units = (int64_t)a.kv.n_seqs * a.blocks * a.kv.kv_heads * 2;
         kv8_append_kernel<FMT, D><<<blocks_of(units, 8), 256, 0, s>>>(a);
-        return cudaGetLastError();
-    }
-};
-
-struct AttendLaunch {
-    const Kv8AttendArgs& a;
-    cudaStream_t s;
-    template <int FMT, int D>
-    cudaError_t run() {
-        const dim3 grid(min(1024u, blocks_of((int64_t)a.max_new * a.heads, 8)), a.kv.n_seqs);
-        kv8_attend_kernel<FMT, D><<<grid, 256, 0, s>>>(a);
-        if (a.mass_out) {
-            const dim3 mgrid(min(1024u, blocks_of((int64_t)a.kv.max_pages * kKv8Page * a.kv.kv_heads, 8)), a.kv.n_seqs);
-            kv8_mass_kernel<FMT, D><<<mgrid, 256, 0, s>>>(a);
-        }
         return cudaGetLastError();
     }
 };
@@ -557,9 +337,8 @@ struct EvictLaunch {
 
 }  // namespace
 
-cudaError_t launch_kv8_append(const Kv8AppendArgs& a, cudaStream_t s) { return by_shape(a.kv, AppendLaunch{a, s}); }
-cudaError_t launch_kv8_attend(const Kv8AttendArgs& a, cudaStream_t s) { return by_shape(a.kv, AttendLaunch{a, s}); }
-cudaError_t launch_kv8_evict(const Kv8EvictArgs& a, cudaStream_t s) { return by_shape(a.src, EvictLaunch{a, s}); }
+cudaError_t launch_kv8_append(const Kv8AppendArgs& a, cudaStream_t s) { return kv8_by_shape(a.kv, AppendLaunch{a, s}); }
+cudaError_t launch_kv8_evict(const Kv8EvictArgs& a, cudaStream_t s) { return kv8_by_shape(a.src, EvictLaunch{a, s}); }
 
 cudaError_t launch_kv8_read(const Kv8ReadArgs& a, cudaStream_t s) {
     const int64_t total = (int64_t)a.kv.n_seqs * a.n * a.kv.kv_heads * (a.kv.head_dim / 8);

@@ -30,8 +30,16 @@ struct Kv8AttendArgs {
     const float* mass_in;
     float* mass_out;
     int64_t mass_stride;
-    float* lse;  // [rows, heads]: log of each softmax's sum, what the weights are rebuilt from
+    // workspace (kv8_attend_workspace)
+    int64_t* offset;  // [n_seqs + 1]: where each sequence's work starts in the list, the list's length
+    float* part;      // partial results of units cut between shares
+    float* lse;       // [rows, heads]: log2 of each softmax's sum, what the weights are rebuilt from; NULL without them
+    int32_t groups;   // shares of the list
 };
+
+// bytes of workspace; with `a`, its pointers into the workspace at `base`
+size_t kv8_attend_workspace(const lastro_kv8& kv, int heads, int max_new, bool with_mass, Kv8AttendArgs* a, void* base);
+
 
 struct Kv8EvictArgs {
     lastro_kv8 src, dst;

@@ -94,8 +94,8 @@ extern "C" int lastro_kv8_attend_workspace(lastro_ctx* ctx, const lastro_kv8* kv
     if (!bytes || heads < 1 || heads % kv->kv_heads || max_new < 0)
         return set_err(ctx, LASTRO_E_ARG, "kv8_attend_workspace: heads %d of %d KV heads, max_new %d", heads, kv->kv_heads,
                        max_new);
-    (void)with_mass;
-    *bytes = std::max<size_t>(16, (size_t)kv->n_seqs * max_new * heads * sizeof(float));
+    KV8_TRY(on_device(ctx, "kv8_attend_workspace"));
+    *bytes = kv8_attend_workspace(*kv, heads, max_new, with_mass != 0, nullptr, nullptr);
     return LASTRO_OK;
 }
 
@@ -136,8 +136,12 @@ extern "C" int lastro_kv8_attend(lastro_ctx* ctx, const lastro_kv8* kv, const in
     a.mass_in = mass_in;
     a.mass_out = mass_out;
     a.mass_stride = mass_stride;
-    a.lse = static_cast<float*>(workspace);
-    if (max_new == 0 && !mass_out) return LASTRO_OK;
+    kv8_attend_workspace(*kv, heads, max_new, mass_out != nullptr, &a, workspace);
+    if (q->rows == 0 && !mass_out) return LASTRO_OK;
+    // the list of work and its shares are counted in 63 and 31 bits
+    if ((int64_t)max_new * a.group >= (1 << 30) || (double)kv->n_seqs * kv->max_pages * 2.0 * heads * max_new >= 1e11)
+        return set_err(ctx, LASTRO_E_UNSUPPORTED, "kv8_attend: n_seqs %d, max_pages %d, max_new %d, heads %d in one call",
+                       kv->n_seqs, kv->max_pages, max_new, heads);
     KV8_TRY(on_device(ctx, "kv8_attend"));
     return launched(ctx, launch_kv8_attend(a, ctx->stream), "kv8_attend");
 }

@@ -26,7 +26,7 @@ DTYPE_BF16, DTYPE_F32, DTYPE_Q8_0 = 1, 2, 3
 LEGACY_STREAM = 1  # cudaStreamLegacy: a Context on the default stream (0 and None make a stream of the context's own)
 KV8_FORMATS = {"e4m3": 1, "int8": 2}
 KV8_PAGE, KV8_BLOCK = 64, 16
-KV8_BAD_PAGE, KV8_BAD_LENGTH, KV8_BAD_OFFSET = 1, 2, 3
+KV8_BAD_PAGE, KV8_BAD_LENGTH, KV8_BAD_OFFSET, KV8_BAD_WAIT = 1, 2, 3, 4
 
 _lib = None
 
