@@ -31,14 +31,17 @@ struct Kv8AttendArgs {
     float* mass_out;
     int64_t mass_stride;
     // workspace (kv8_attend_workspace)
-    int64_t* offset;  // [n_seqs + 1]: where each sequence's work starts in the list, the list's length
-    float* part;      // partial results of units cut between shares
-    float* lse;       // [rows, heads]: log2 of each softmax's sum, what the weights are rebuilt from; NULL without them
-    int32_t groups;   // shares of the list
+    int32_t* offset;       // [n_seqs + 1]: where each sequence's work starts in the list, the list's length
+    float* part;           // partial results of units cut between shares of the list
+    float* lse;            // [rows, heads]: log2 of each softmax's sum, what the weights are rebuilt from; NULL without them
+    float* scores;         // [list items][score_rows][chunk's slots]: the scores, where they are kept
+    int32_t shares, score_rows;
 };
 
 // bytes of workspace; with `a`, its pointers into the workspace at `base`
 size_t kv8_attend_workspace(const lastro_kv8& kv, int heads, int max_new, bool with_mass, Kv8AttendArgs* a, void* base);
+// the longest list of work a call can have
+int64_t kv8_attend_items(const lastro_kv8& kv, int heads, int max_new);
 
 
 struct Kv8EvictArgs {

@@ -138,8 +138,7 @@ extern "C" int lastro_kv8_attend(lastro_ctx* ctx, const lastro_kv8* kv, const in
     a.mass_stride = mass_stride;
     kv8_attend_workspace(*kv, heads, max_new, mass_out != nullptr, &a, workspace);
     if (q->rows == 0 && !mass_out) return LASTRO_OK;
-    // the list of work and its shares are counted in 63 and 31 bits
-    if ((int64_t)max_new * a.group >= (1 << 30) || (double)kv->n_seqs * kv->max_pages * 2.0 * heads * max_new >= 1e11)
+    if ((int64_t)max_new * a.heads > INT32_MAX || kv8_attend_items(*kv, heads, max_new) >= (1 << 30))  // counted in 32 bits
         return set_err(ctx, LASTRO_E_UNSUPPORTED, "kv8_attend: n_seqs %d, max_pages %d, max_new %d, heads %d in one call",
                        kv->n_seqs, kv->max_pages, max_new, heads);
     KV8_TRY(on_device(ctx, "kv8_attend"));
