@@ -50,9 +50,13 @@ __global__ void __launch_bounds__(256) kv8_append_kernel(const __grid_constant__
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         const int r = r0 + i * RPW;
-        if (r >= beg && r < end)
-            load8(src, (int64_t)(first + slot0 + r - len) * src.row_stride + h * src.head_stride + c, vec, x[i]);
-        else
+        if (r >= beg && r < end) {
+            const int64_t at = (int64_t)(first + slot0 + r - len) * src.row_stride + h * src.head_stride + c;
+            if (src.dtype == LASTRO_DTYPE_F32)
+                load8<true>(src, at, vec, x[i]);
+            else
+                load8<false>(src, at, vec, x[i]);
+        } else
 #pragma unroll
             for (int q = 0; q < 8; ++q) x[i][q] = 0.0f;
 #pragma unroll

@@ -79,8 +79,9 @@ LDEV void decode4(uint32_t w, float (&v)[4]) {
 }
 
 // 8 consecutive values of an activation row; `vec`: every such group is 16-byte aligned
+template <bool F32>
 LDEV void load8(const lastro_rows& r, int64_t at, bool vec, float (&v)[8]) {
-    if (r.dtype == LASTRO_DTYPE_F32) {
+    if (F32) {
         const float* p = static_cast<const float*>(r.ptr) + at;
         if (vec) {
             const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
