@@ -8,18 +8,17 @@ namespace lastro {
 namespace {
 
 // ---- append ---------------------------------------------------------------------------------------------------------
-// One warp quantises one block (16 slots) of K or V of one head: its new rows pass through registers once (a lane holds
-// groups of 8 values), the largest magnitude by a warp reduction, then the codes.  The block's earlier rows are read and
-// rounded again only where the scale grows.
-template <int FMT, int D>
+// One warp quantises one block (16 slots) of K and V of one head: its new rows are read once into registers (a lane holds
+// groups of 8 values), the largest magnitude comes by a warp reduction, then the codes.  The block's earlier rows are read
+// and rounded again only where the scale grows.  Bound by memory: 2 or 4 bytes a value in, 1 out.
+template <int FMT, int D, bool F32>
 __global__ void __launch_bounds__(256) kv8_append_kernel(const __grid_constant__ Kv8AppendArgs a) {
     constexpr int LPR = D / 8, RPW = 32 / LPR, N = kKv8Block / RPW;  // lanes a row, rows a pass, passes
-    const int64_t unit = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-    const int lane = threadIdx.x & 31, H = a.kv.kv_heads;
-    const int which = (int)(unit & 1), h = (int)((unit >> 1) % H);
-    const int64_t bj = (unit >> 1) / H;
-    const int b = (int)(bj / a.blocks), j = (int)(bj % a.blocks);
-    if (b >= a.kv.n_seqs) return;
+    pdl_wait();
+    pdl_launch();
+    const int lane = threadIdx.x & 31, H = a.kv.kv_heads, b = blockIdx.y;
+    const int unit = blockIdx.x * 8 + (threadIdx.x >> 5), j = unit / H, h = unit - j * H;
+    if (j >= a.blocks) return;
     int64_t most = (int64_t)a.kv.max_pages * kKv8Page;
     if (a.mass) most = min(most, a.mass_stride);
     const int len = seq_len(a.kv, a.lens, b, most);
@@ -28,7 +27,7 @@ __global__ void __launch_bounds__(256) kv8_append_kernel(const __grid_constant__
         if (n > most - len) report(a.kv, LASTRO_KV8_BAD_LENGTH);
         n = 0;
     }
-    if (which == 0 && j == 0) {
+    if (j == 0) {
         if (h == 0 && lane == 0) a.lens_out[b] = len + n;
         if (a.mass)
             for (int i = lane; i < n; i += 32) a.mass[((int64_t)b * H + h) * a.mass_stride + len + i] = 0.0f;
@@ -39,100 +38,126 @@ __global__ void __launch_bounds__(256) kv8_append_kernel(const __grid_constant__
     if (page < 0) return;
     const int beg = max(0, len - slot0), end = min(kKv8Block, len + n - slot0);  // its new rows
     const int64_t tile = (int64_t)page * H + h;
-    uint8_t* codes = static_cast<uint8_t*>(which ? a.kv.v : a.kv.k) + (tile * kKv8Page + slot0 % kKv8Page) * D;
-    float* scale = (which ? a.kv.v_scale : a.kv.k_scale) + tile * kKv8Blocks + slot0 % kKv8Page / kKv8Block;
-    const lastro_rows& src = which ? a.v : a.k;
-    const bool vec = vec_rows(src);
+    const int64_t code0 = (tile * kKv8Page + slot0 % kKv8Page) * D, block = tile * kKv8Blocks + slot0 % kKv8Page / kKv8Block;
     const int r0 = lane / LPR, c = lane % LPR * 8;
 
-    float x[N][8];
-    uint32_t amax = 0;
+    auto fetch = [&](const lastro_rows& src, Raw8<F32> (&x)[N]) {
+        const bool vec = vec_rows(src);
+        const int64_t base = (int64_t)(first + slot0 - len) * src.row_stride + h * src.head_stride + c;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const int r = r0 + i * RPW;
-        if (r >= beg && r < end) {
-            const int64_t at = (int64_t)(first + slot0 + r - len) * src.row_stride + h * src.head_stride + c;
-            if (src.dtype == LASTRO_DTYPE_F32)
-                load8<true>(src, at, vec, x[i]);
+        for (int i = 0; i < N; ++i) {
+            const int r = r0 + i * RPW;
+            if (r >= beg && r < end)
+                x[i].load(src, base + r * src.row_stride, vec);
             else
-                load8<false>(src, at, vec, x[i]);
-        } else
-#pragma unroll
-            for (int q = 0; q < 8; ++q) x[i][q] = 0.0f;
-#pragma unroll
-        for (int q = 0; q < 8; ++q) amax = max(amax, __float_as_uint(x[i][q]) & 0x7fffffffu);
-    }
-    float s = scale_for<FMT>(warp_umax(amax));
-    const float was = beg ? *scale : s;
-    if (was != was || (s == s && was > s)) s = was;  // earlier rows: the larger scale, NaN stays
-    const bool nan = s != s;
-    const float inv = nan ? 0.0f : inverse(s);
-    __syncwarp();  // every lane has read the old scale
-    if (lane == 0) *scale = s;
-    const bool again = beg && (nan || was != s);
-    const float ratio = nan ? 0.0f : was * inv;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const int r = r0 + i * RPW;
-        uint2* dst = reinterpret_cast<uint2*>(codes + r * D + c);
-        if (r >= beg && r < end) {
-            if (nan)
-#pragma unroll
-                for (int q = 0; q < 8; ++q) x[i][q] = 0.0f;
-            uint2 o;
-            o.x = encode4<FMT>(x[i][0] * inv, x[i][1] * inv, x[i][2] * inv, x[i][3] * inv);
-            o.y = encode4<FMT>(x[i][4] * inv, x[i][5] * inv, x[i][6] * inv, x[i][7] * inv);
-            *dst = o;
-        } else if (again && r < beg) {
-            const uint2 w = *dst;
-            float u[4], t[4];
-            decode4<FMT>(w.x, u);
-            decode4<FMT>(w.y, t);
-            *dst = make_uint2(encode4<FMT>(u[0] * ratio, u[1] * ratio, u[2] * ratio, u[3] * ratio),
-                              encode4<FMT>(t[0] * ratio, t[1] * ratio, t[2] * ratio, t[3] * ratio));
+                x[i].zero();
         }
+    };
+    auto put = [&](uint8_t* codes, float* scale, float was, const Raw8<F32> (&x)[N]) {
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i].widest(m);
+        float s = scale_for<FMT>(warp_umax(Raw8<F32>::f32_bits(m)));
+        if (beg && (was != was || was > s)) s = was;  // earlier rows: the larger scale, and NaN stays
+        const bool nan = s != s;
+        const float inv = nan ? 0.0f : inverse(s);
+        const bool again = beg && (nan || was != s);
+        if (lane == 0) *scale = s;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int r = r0 + i * RPW;
+            uint2* dst = reinterpret_cast<uint2*>(codes + r * D + c);
+            if (r >= beg && r < end) {
+                float v[8];
+                x[i].values(v);
+                uint2 o = make_uint2(0, 0);
+                if (!nan) o = make_uint2(encode4<FMT>(v[0], v[1], v[2], v[3], inv), encode4<FMT>(v[4], v[5], v[6], v[7], inv));
+                *dst = o;
+            } else if (again && r < beg) {
+                const uint2 w = *dst;
+                float u[4], t[4];
+                decode4<FMT>(w.x, u);
+                decode4<FMT>(w.y, t);
+                const float ratio = nan ? 0.0f : was * inv;
+                *dst = make_uint2(encode4<FMT>(u[0], u[1], u[2], u[3], ratio), encode4<FMT>(t[0], t[1], t[2], t[3], ratio));
+            }
+        }
+    };
+    uint8_t *kc = static_cast<uint8_t*>(a.kv.k) + code0, *vc = static_cast<uint8_t*>(a.kv.v) + code0;
+    const float kwas = a.kv.k_scale[block], vwas = a.kv.v_scale[block];
+    Raw8<F32> x[N];
+    if (F32) {  // K and V one after the other: both would not fit the registers
+        fetch(a.k, x);
+        put(kc, a.kv.k_scale + block, kwas, x);
+        fetch(a.v, x);
+        put(vc, a.kv.v_scale + block, vwas, x);
+    } else {
+        Raw8<F32> y[N];
+        fetch(a.k, x);
+        fetch(a.v, y);
+        put(kc, a.kv.k_scale + block, kwas, x);
+        put(vc, a.kv.v_scale + block, vwas, y);
     }
 }
 
 // ---- read-back ------------------------------------------------------------------------------------------------------
-template <int FMT, bool F32>
-__global__ void __launch_bounds__(256) kv8_read_kernel(const __grid_constant__ Kv8ReadArgs a) {
-    const int H = a.kv.kv_heads, D = a.kv.head_dim, G = D / 8;
-    const int64_t total = (int64_t)a.kv.n_seqs * a.n * H * G;
-    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
-        const int c = (int)(i % G) * 8, h = (int)(i / G % H);
-        const int64_t bj = i / G / H;
-        const int b = (int)(bj / a.n), j = (int)(bj % a.n);
-        const int len = seq_len(a.kv, a.lens, b, (int64_t)a.kv.max_pages * kKv8Page);
-        const int64_t slot = (int64_t)__ldg(a.pos0 + b) + j;
-        const int page = slot >= 0 && slot < len ? page_of(a.kv, b, (int)slot) : -1;
+// One warp takes kReadSlots slots of a sequence, all heads: a lane turns 8 codes into 16 or 32 bytes, so that a warp's stores
+// are whole lines (16 codes a lane, whose stores leave gaps for the next, ran at half the rate).
+constexpr int kReadSlots = 2;
+
+template <int FMT, int D, bool F32>
+__global__ void __launch_bounds__(256, 5) kv8_read_kernel(const __grid_constant__ Kv8ReadArgs a) {
+    constexpr int LPR = D / 8, HPW = 32 / LPR;  // lanes a row, heads a pass
+    pdl_wait();
+    pdl_launch();
+    const int lane = threadIdx.x & 31, H = a.kv.kv_heads, b = blockIdx.y;
+    const int j0 = (blockIdx.x * 8 + (threadIdx.x >> 5)) * kReadSlots;
+    if (j0 >= a.n) return;
+    const int len = seq_len(a.kv, a.lens, b, (int64_t)a.kv.max_pages * kKv8Page);
+    const int64_t pos0 = (int64_t)__ldg(a.pos0 + b) + j0;
+    int page[kReadSlots];
 #pragma unroll
-        for (int which = 0; which < 2; ++which) {
-            void* out = which ? a.v_out : a.k_out;
-            if (!out) continue;
-            float v[8] = {};
-            if (page >= 0) {
-                const int64_t tile = (int64_t)page * H + h;
-                const uint8_t* codes = static_cast<const uint8_t*>(which ? a.kv.v : a.kv.k);
-                const uint2 w = __ldg(reinterpret_cast<const uint2*>(codes + (tile * kKv8Page + slot % kKv8Page) * D + c));
-                const float s = __ldg((which ? a.kv.v_scale : a.kv.k_scale) + tile * kKv8Blocks + slot % kKv8Page / kKv8Block);
-                float lo[4], hi[4];
-                decode4<FMT>(w.x, lo);
-                decode4<FMT>(w.y, hi);
+    for (int i = 0; i < kReadSlots; ++i)
+        page[i] = j0 + i < a.n && pos0 + i >= 0 && pos0 + i < len ? page_of(a.kv, b, (int)(pos0 + i)) : -1;
+    for (int h0 = 0; h0 < H; h0 += HPW) {
+        const int h = h0 + lane / LPR, c = lane % LPR * 8;
+        if (h >= H) continue;
+        uint2 w[2][kReadSlots];
+        float s[2][kReadSlots];
 #pragma unroll
-                for (int q = 0; q < 4; ++q) v[q] = lo[q] * s, v[4 + q] = hi[q] * s;
+        for (int i = 0; i < kReadSlots; ++i) {
+            const int row = (int)((pos0 + i) & (kKv8Page - 1));
+            const int64_t tile = (int64_t)page[i] * H + h;
+#pragma unroll
+            for (int v = 0; v < 2; ++v) {
+                w[v][i] = make_uint2(0, 0);
+                s[v][i] = 0.0f;
+                if (page[i] >= 0 && (v ? a.v_out : a.k_out)) {
+                    w[v][i] = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(v ? a.kv.v : a.kv.k) + (tile * kKv8Page + row) * D + c));
+                    s[v][i] = __ldg((v ? a.kv.v_scale : a.kv.k_scale) + tile * kKv8Blocks + row / kKv8Block);
+                }
             }
-            if (F32) {
-                float4* dst = reinterpret_cast<float4*>(static_cast<float*>(out) + i * 8);
-                dst[0] = make_float4(v[0], v[1], v[2], v[3]);
-                dst[1] = make_float4(v[4], v[5], v[6], v[7]);
-            } else {
-                uint4 o;
-                o.x = pack_bf16(f32_to_bf16_rne(v[0]), f32_to_bf16_rne(v[1]));
-                o.y = pack_bf16(f32_to_bf16_rne(v[2]), f32_to_bf16_rne(v[3]));
-                o.z = pack_bf16(f32_to_bf16_rne(v[4]), f32_to_bf16_rne(v[5]));
-                o.w = pack_bf16(f32_to_bf16_rne(v[6]), f32_to_bf16_rne(v[7]));
-                reinterpret_cast<uint4*>(out)[i] = o;
+        }
+#pragma unroll
+        for (int i = 0; i < kReadSlots; ++i) {
+            if (j0 + i >= a.n) break;
+            const int64_t at = (((int64_t)b * a.n + j0 + i) * H + h) * D + c;
+#pragma unroll
+            for (int v = 0; v < 2; ++v) {
+                void* out = v ? a.v_out : a.k_out;
+                if (!out) continue;
+                float x[4], y[4];
+                decode4<FMT>(w[v][i].x, x);
+                decode4<FMT>(w[v][i].y, y);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) x[k] *= s[v][i], y[k] *= s[v][i];
+                if (F32) {
+                    reinterpret_cast<float4*>(static_cast<float*>(out) + at)[0] = make_float4(x[0], x[1], x[2], x[3]);
+                    reinterpret_cast<float4*>(static_cast<float*>(out) + at)[1] = make_float4(y[0], y[1], y[2], y[3]);
+                } else {
+                    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(out) + at) =
+                        make_uint4(two_bf16(x[0], x[1]), two_bf16(x[2], x[3]), two_bf16(y[0], y[1]), two_bf16(y[2], y[3]));
+                }
             }
         }
     }
@@ -146,42 +171,49 @@ LDEV uint32_t mass_key(float m) {
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-constexpr int kSelThreads = 1024;
+LDEV float key_mass(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
 
-// exclusive prefix sum of v over the block and the total; `red` holds 33 ints
-LDEV int block_scan(int v, int* red, int& total) {
-    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-    int s = v;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int t = __shfl_up_sync(0xffffffffu, s, o);
-        if (lane >= o) s += t;
-    }
-    __syncthreads();
-    if (lane == 31) red[w] = s;
-    __syncthreads();
-    if (w == 0) {
-        int x = red[lane];
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int t = __shfl_up_sync(0xffffffffu, x, o);
-            if (lane >= o) x += t;
-        }
-        red[lane] = x;
-    }
-    __syncthreads();
-    total = red[31];
-    return s - v + (w ? red[w - 1] : 0);
+constexpr int kSelSlots = 16384;  // slots whose keys a CTA keeps in shared memory, after its histograms
+constexpr int kSelBins = 4096;
+
+LDEV void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.aligned;\nbarrier.cluster.wait.aligned;" ::: "memory");
+}
+LDEV uint32_t cluster_rank() {
+    uint32_t r;
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+// adds to a word of CTA `rank`'s shared memory, at the address `p` has in this one
+LDEV void add_cluster(uint32_t* p, uint32_t rank, uint32_t v) {
+    uint32_t a;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_addr(p)), "r"(rank));
+    asm volatile("red.relaxed.cluster.shared::cluster.add.u32 [%0], %1;" ::"r"(a), "r"(v) : "memory");
+}
+// such a word
+LDEV uint32_t ld_cluster(const uint32_t* p, uint32_t rank) {
+    uint32_t a, v;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_addr(p)), "r"(rank));
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(a));
+    return v;
 }
 
-// One CTA per sequence and KV head: the key of the (budget - recent)-th largest mass by four 8-bit radix passes, then one
-// pass that writes the kept slots in order (all above the key, and of those at it the lowest slots).
-__global__ void __launch_bounds__(kSelThreads) kv8_select_kernel(const __grid_constant__ Kv8EvictArgs a) {
-    __shared__ uint32_t hist[256];
-    __shared__ int red[33];
-    __shared__ uint32_t s_key;
-    __shared__ int s_need;
-    const int H = a.src.kv_heads, h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, C = a.budget;
+// One cluster of CL CTAs per sequence and KV head, each with an equal run of the slots that may be dropped, whose keys it
+// holds in shared memory: the key of the (budget - recent)-th largest mass by three radix passes (12, 10 and 10 bits; masses
+// share their leading bits, and 8-bit digits had most of them counted in a few words, one at a time) over histograms, whose
+// counts every CTA adds to all the others' (few are not zero), then one pass that writes the kept slots in order (all above the key, and of those at it the
+// lowest slots): a warp takes consecutive slots and knows from counts what is kept before them.
+template <int CL>
+__global__ void __launch_bounds__(CL > 1 ? 1024 : 512) kv8_select_kernel(const __grid_constant__ Kv8EvictArgs a) {
+    constexpr int kSelThreads = CL > 1 ? 1024 : 512, kSelWarps = kSelThreads / 32;
+    extern __shared__ uint32_t room[];
+    // this CTA's counts; with a cluster, two arrays of everybody's besides, one cleared while the other is added to
+    uint32_t *hist = room, *both = room + kSelBins, *keys = room + (CL > 1 ? 3 : 1) * kSelBins;
+    __shared__ uint32_t part[kSelWarps], found[2], above[kSelWarps + 1], ties[kSelWarps + 1];
+    pdl_wait();
+    pdl_launch();
+    const int H = a.src.kv_heads, b = blockIdx.z, h = blockIdx.y, tid = threadIdx.x, C = a.budget;
+    const int lane = tid & 31, warp = tid >> 5, rank = CL > 1 ? (int)cluster_rank() : 0, all = CL * kSelThreads, me = rank * kSelThreads + tid;
     int64_t most = (int64_t)a.src.max_pages * kKv8Page;
     if (a.mass) most = min(most, a.mass_stride);
     const int len = seq_len(a.src, a.lens, b, most);
@@ -190,126 +222,254 @@ __global__ void __launch_bounds__(kSelThreads) kv8_select_kernel(const __grid_co
     const float* mass = a.mass ? a.mass + seq * a.mass_stride : nullptr;
     float* mout = a.mass_out ? a.mass_out + seq * a.mass_out_stride : nullptr;
     const int keep = min(len, C);
-    if (h == 0 && tid == 0) a.lens_out[b] = keep;
-    for (int i = keep + tid; i < C; i += kSelThreads) kept[i] = -1;
-    if (len <= C) {
-        for (int i = tid; i < len; i += kSelThreads) {
-            kept[i] = i;
-            if (mout) mout[i] = mass ? mass[i] : 0.0f;
-        }
-        return;
-    }
-    const int cand = len - a.recent, want = C - a.recent;  // cand > want
-    if (want > 0) {
-        uint32_t prefix = 0;
-        int need = want;
-        for (int shift = 24; shift >= 0; shift -= 8) {
-            if (tid < 256) hist[tid] = 0;
-            __syncthreads();
-            const uint32_t mask = shift == 24 ? 0u : 0xffffffffu << (shift + 8);
-            for (int t = tid; t < cand; t += kSelThreads) {
-                const uint32_t k = mass_key(mass[t]);
-                if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & 255], 1u);
-            }
-            __syncthreads();
-            if (tid == 0) {
-                int left = need, d = 255;
-                for (; d > 0 && (int)hist[d] < left; --d) left -= hist[d];
-                s_key = prefix | (uint32_t)d << shift;
-                s_need = left;
-            }
-            __syncthreads();
-            prefix = s_key;
-            need = s_need;
-        }
-        // `need` of the slots whose key equals prefix are kept
-        int ties = 0, out = 0;
-        for (int base = 0; base < cand; base += kSelThreads) {
-            const int t = base + tid;
-            const float m = t < cand ? mass[t] : 0.0f;
-            const uint32_t k = mass_key(m);
-            const bool tie = t < cand && k == prefix;
-            int nt, ns;
-            const int rank = ties + block_scan(tie, red, nt);
-            const bool sel = t < cand && (k > prefix || (tie && rank < need));
-            const int at = out + block_scan(sel, red, ns);
-            if (sel) {
-                kept[at] = t;
-                if (mout) mout[at] = m;
-            }
-            ties += nt;
-            out += ns;
-        }
-    }
-    for (int i = tid; i < a.recent; i += kSelThreads) {
+    if (h == 0 && me == 0) a.lens_out[b] = keep;
+    for (int i = keep + me; i < C; i += all) kept[i] = -1;
+    // the slots kept whatever their mass: all, or the last `recent`
+    const int want = len <= C ? 0 : C - a.recent, cand = len <= C ? 0 : len - a.recent;
+    for (int i = me; i < keep - want; i += all) {
         kept[want + i] = cand + i;
-        if (mout) mout[want + i] = mass ? mass[cand + i] : 0.0f;
+        if (mout) mout[want + i] = mass[cand + i];
     }
+    if (want == 0) return;  // the same for the whole cluster
+
+    const int run = ((cand + CL - 1) / CL + 3) & ~3, lo = min(cand, rank * run), n = min(cand, lo + run) - lo;
+    const bool held = run <= kSelSlots;
+    if (held && (reinterpret_cast<uintptr_t>(mass) & 15) == 0) {
+#pragma unroll 4
+        for (int i = tid; i < n / 4; i += kSelThreads) {
+            const float4 m = __ldg(reinterpret_cast<const float4*>(mass + lo) + i);
+            reinterpret_cast<uint4*>(keys)[i] = make_uint4(mass_key(m.x), mass_key(m.y), mass_key(m.z), mass_key(m.w));
+        }
+        if (tid < (n & 3)) keys[n - 1 - tid] = mass_key(__ldg(mass + lo + n - 1 - tid));
+        __syncthreads();
+    } else if (held) {
+#pragma unroll 8
+        for (int i = tid; i < n; i += kSelThreads) keys[i] = mass_key(__ldg(mass + lo + i));
+    }
+    auto key = [&](int i) { return held ? keys[i] : mass_key(__ldg(mass + lo + i)); };
+    if (CL > 1) {
+        for (int i = tid; i < kSelBins; i += kSelThreads) both[i] = 0;
+        cluster_sync();
+    }
+    uint32_t prefix = 0, need = want;
+#pragma unroll 1
+    for (int pass = 0; pass < 3; ++pass) {
+        const int shift = pass == 0 ? 20 : pass == 1 ? 10 : 0, bins = pass == 0 ? kSelBins : 1024;
+        const uint32_t* total = CL > 1 ? both + (pass & 1) * kSelBins : hist;
+        for (int i = tid; i < bins; i += kSelThreads) hist[i] = 0;
+        __syncthreads();
+        const uint32_t mask = pass == 0 ? 0u : pass == 1 ? 0xfff00000u : 0xfffffc00u;
+#pragma unroll 8
+        for (int i = tid; i < n; i += kSelThreads) {
+            const uint32_t k = key(i);
+            if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & (bins - 1)], 1u);
+        }
+        __syncthreads();
+        if (CL > 1) {
+            uint32_t* next = both + (~pass & 1) * kSelBins;
+            for (int i = tid; i < bins; i += kSelThreads) {
+                const uint32_t c = hist[i];
+                if (c)
+                    for (int r = 0; r < CL; ++r) add_cluster(both + (pass & 1) * kSelBins + i, r, c);
+            }
+            for (int i = tid; i < 1024; i += kSelThreads) next[i] = 0;  // the later passes' bins
+            cluster_sync();
+        }
+        // thread t's digits, from the largest down: bins - 1 - per t and the per - 1 below it
+        const int per = max(1, bins / kSelThreads);
+        uint32_t c[kSelBins / kSelThreads], sum = 0;
+#pragma unroll
+        for (int i = 0; i < kSelBins / kSelThreads; ++i) {
+            const int d = bins - 1 - (tid * per + i);
+            c[i] = i < per && d >= 0 ? total[d] : 0u;
+            sum += c[i];
+        }
+        uint32_t incl = sum;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t t = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += t;
+        }
+        if (lane == 31) part[warp] = incl;
+        __syncthreads();
+        uint32_t before = __reduce_add_sync(0xffffffffu, lane < warp ? part[lane & (kSelWarps - 1)] : 0u) + incl - sum;
+        if (before < need && need <= before + sum) {  // one thread: the digit that the last wanted slot has
+            bool done = false;
+#pragma unroll
+            for (int i = 0; i < kSelBins / kSelThreads; ++i) {
+                if (!done && before + c[i] >= need) {
+                    found[0] = prefix | (uint32_t)(bins - 1 - (tid * per + i)) << shift;
+                    found[1] = need - before;
+                    done = true;
+                }
+                if (!done) before += c[i];
+            }
+        }
+        __syncthreads();
+        prefix = found[0];
+        need = found[1];
+    }
+    // kept: every key above prefix, and the first `need` at it
+    const int span = ((n + kSelWarps - 1) / kSelWarps + 31) & ~31, wlo = min(n, warp * span), whi = min(n, wlo + span);
+    uint32_t up = 0, at = 0;
+    for (int i = wlo + lane; i < whi; i += 32) {
+        const uint32_t k = key(i);
+        up += k > prefix;
+        at += k == prefix;
+    }
+    up = __reduce_add_sync(0xffffffffu, up);
+    at = __reduce_add_sync(0xffffffffu, at);
+    if (lane == 0) above[warp] = up, ties[warp] = at;
+    __syncthreads();
+    // what is kept before this warp's slots: in the CTA's earlier warps, and in the cluster's earlier CTAs
+    const uint32_t wu = lane < kSelWarps ? above[lane] : 0u, wt = lane < kSelWarps ? ties[lane] : 0u;
+    up = __reduce_add_sync(0xffffffffu, lane < warp ? wu : 0u);
+    at = __reduce_add_sync(0xffffffffu, lane < warp ? wt : 0u);
+    if (CL > 1) {
+        const uint32_t u = __reduce_add_sync(0xffffffffu, wu), t = __reduce_add_sync(0xffffffffu, wt);
+        if (tid == 0) above[kSelWarps] = u, ties[kSelWarps] = t;
+        cluster_sync();
+        up += __reduce_add_sync(0xffffffffu, lane < rank ? ld_cluster(&above[kSelWarps], lane) : 0u);
+        at += __reduce_add_sync(0xffffffffu, lane < rank ? ld_cluster(&ties[kSelWarps], lane) : 0u);
+    }
+    for (int i0 = wlo; i0 < whi; i0 += 32) {
+        const int i = i0 + lane;
+        const uint32_t k = i < whi ? key(i) : 0u;
+        const unsigned gt = __ballot_sync(0xffffffffu, i < whi && k > prefix), eq = __ballot_sync(0xffffffffu, i < whi && k == prefix);
+        const unsigned below = (1u << lane) - 1;
+        const uint32_t u = up + __popc(gt & below), t = at + __popc(eq & below);
+        if ((gt >> lane & 1) || ((eq >> lane & 1) && t < need)) {
+            const uint32_t pos = u + min(t, need);
+            kept[pos] = lo + i;
+            if (mout) mout[pos] = key_mass(k);
+        }
+        up += __popc(gt);
+        at += __popc(eq);
+    }
+    if (CL > 1) cluster_sync();  // no CTA leaves while another reads its counts
 }
 
-// One warp gathers one destination block of K or V: 16 kept rows, their largest magnitude, the new scale and codes.
+// four codes as two f16 pairs, exactly, and back (what they are multiplied by keeps them in the format's range)
+template <int FMT>
+LDEV void to_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
+    if (FMT == E4M3) {
+        asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(lo) : "h"((uint16_t)w));
+        asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(hi) : "h"((uint16_t)(w >> 16)));
+    } else {  // f16 0x6400 + u is 1024 + u for a byte u = code + 128
+        const uint32_t u = w ^ 0x80808080u, bias = 0x64806480u;
+        asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(lo) : "r"(__byte_perm(u, 0x64646464u, 0x4140)), "r"(bias));
+        asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(hi) : "r"(__byte_perm(u, 0x64646464u, 0x4342)), "r"(bias));
+    }
+}
+template <int FMT>
+LDEV uint32_t from_f16(uint32_t lo, uint32_t hi) {
+    if (FMT == E4M3) {
+        uint16_t a, b;
+        asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(a) : "r"(lo));
+        asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(b) : "r"(hi));
+        return a | (uint32_t)b << 16;
+    }
+    uint32_t a, b;  // 1536 + x rounds x to a whole number, whose low byte is the f16's
+    asm("add.rn.f16x2 %0, %1, %2;" : "=r"(a) : "r"(lo), "r"(0x66006600u));
+    asm("add.rn.f16x2 %0, %1, %2;" : "=r"(b) : "r"(hi), "r"(0x66006600u));
+    return __byte_perm(a, b, 0x6420);
+}
+LDEV uint32_t mul_f16(uint32_t x, uint32_t y) {
+    uint32_t r;
+    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(y));
+    return r;
+}
+
+// One warp gathers kGatherBlocks destination blocks of K and V of one head: their kept rows as 16-byte pieces, all on
+// their way before the first is used (a row takes three dependent loads: the slot kept, its page, the codes), then for each
+// block the largest magnitude, the new scale, and the codes times a ratio of powers of two, in f16 (a code has at most 8
+// significant bits).  Bound by memory: each kept row is read and written once.
+constexpr int kGatherBlocks = 2;
+
 template <int FMT, int D>
 __global__ void __launch_bounds__(256) kv8_gather_kernel(const __grid_constant__ Kv8EvictArgs a) {
-    constexpr int LPR = D / 8, RPW = 32 / LPR, N = kKv8Block / RPW;
-    const int lane = threadIdx.x & 31, H = a.src.kv_heads, blocks = (a.budget + kKv8Block - 1) / kKv8Block;
-    const int64_t unit = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-    const int which = (int)(unit & 1), j = (int)((unit >> 1) % blocks);
-    const int64_t seq = (unit >> 1) / blocks;
-    const int b = (int)(seq / H), h = (int)(seq % H);
-    if (b >= a.src.n_seqs) return;
-    const int keep = a.lens_out[b], slot0 = j * kKv8Block;
+    constexpr int LPR = D / 16, RPW = 32 / LPR, N = kKv8Block / RPW;  // lanes a row, rows a pass, passes
+    static_assert(kGatherBlocks * kKv8Block == 32, "a lane for each row");
+    pdl_wait();
+    pdl_launch();
+    const int lane = threadIdx.x & 31, H = a.src.kv_heads, h = blockIdx.y, b = blockIdx.z;
+    const int slot0 = (blockIdx.x * 8 + (threadIdx.x >> 5)) * 32;
+    const int keep = __ldcg(a.lens_out + b);
     if (slot0 >= keep) return;
-    if (keep > (int64_t)a.dst.max_pages * kKv8Page) {
-        report(a.dst, LASTRO_KV8_BAD_LENGTH);
-        return;
+    const int dpage = page_of(a.dst, b, slot0);  // both blocks are in one page
+    // lane r: where kept row r is, and its scales
+    int64_t from = -1;
+    float ks = 0.0f, vs = 0.0f;
+    if (slot0 + lane < keep) {
+        const int t = __ldcg(a.kept + ((int64_t)b * H + h) * a.budget + slot0 + lane), page = page_of(a.src, b, t);
+        if (page >= 0) {
+            const int64_t tile = (int64_t)page * H + h;
+            from = tile * kKv8Page + t % kKv8Page;
+            ks = __ldg(a.src.k_scale + tile * kKv8Blocks + t % kKv8Page / kKv8Block);
+            vs = __ldg(a.src.v_scale + tile * kKv8Blocks + t % kKv8Page / kKv8Block);
+        }
     }
-    const int dpage = page_of(a.dst, b, slot0);
     if (dpage < 0) return;
-    const int r0 = lane / LPR, c = lane % LPR * 8;
-    const uint8_t* src = static_cast<const uint8_t*>(which ? a.src.v : a.src.k);
-    const float* sscale = which ? a.src.v_scale : a.src.k_scale;
-    uint2 w[N];
-    float sc[N];
-    uint32_t amax = 0;
+    const int r0 = lane / LPR, c = lane % LPR * 16;
+    uint4 w[kGatherBlocks][2][N];
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const int r = slot0 + r0 + i * RPW;
-        w[i] = make_uint2(0, 0);
-        sc[i] = 0.0f;
-        if (r < keep) {
-            const int t = a.kept[seq * a.budget + r];
-            const int page = page_of(a.src, b, t);
-            if (page >= 0) {
-                const int64_t tile = (int64_t)page * H + h;
-                w[i] = __ldg(reinterpret_cast<const uint2*>(src + (tile * kKv8Page + t % kKv8Page) * D + c));
-                sc[i] = __ldg(sscale + tile * kKv8Blocks + t % kKv8Page / kKv8Block);
+    for (int g = 0; g < kGatherBlocks; ++g)
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int64_t row = __shfl_sync(0xffffffffu, from, g * kKv8Block + r0 + i * RPW);
+            w[g][0][i] = w[g][1][i] = make_uint4(0, 0, 0, 0);
+            if (row >= 0) {
+                w[g][0][i] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(a.src.k) + row * D + c));
+                w[g][1][i] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(a.src.v) + row * D + c));
             }
         }
-        float u[4], v[4];
-        decode4<FMT>(w[i].x, u);
-        decode4<FMT>(w[i].y, v);
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            amax = max(amax, __float_as_uint(u[q] * sc[i]) & 0x7fffffffu);
-            amax = max(amax, __float_as_uint(v[q] * sc[i]) & 0x7fffffffu);
-        }
-    }
-    const float s = scale_for<FMT>(warp_umax(amax));
-    const bool nan = s != s;
-    const float inv = nan ? 0.0f : inverse(s);
     const int64_t tile = (int64_t)dpage * H + h;
-    uint8_t* dst = static_cast<uint8_t*>(which ? a.dst.v : a.dst.k) + (tile * kKv8Page + slot0 % kKv8Page) * D;
-    if (lane == 0) (which ? a.dst.v_scale : a.dst.k_scale)[tile * kKv8Blocks + slot0 % kKv8Page / kKv8Block] = s;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const int r = r0 + i * RPW;
-        if (slot0 + r >= keep) continue;
-        float u[4], v[4];
-        decode4<FMT>(w[i].x, u);
-        decode4<FMT>(w[i].y, v);
-        const float f = nan ? 0.0f : sc[i] * inv;  // a ratio of powers of two
-        *reinterpret_cast<uint2*>(dst + r * D + c) = make_uint2(encode4<FMT>(u[0] * f, u[1] * f, u[2] * f, u[3] * f),
-                                                                encode4<FMT>(v[0] * f, v[1] * f, v[2] * f, v[3] * f));
+    for (int g = 0; g < kGatherBlocks; ++g) {
+        const int first = slot0 + g * kKv8Block;
+        if (first >= keep) return;
+#pragma unroll
+        for (int v = 0; v < 2; ++v) {
+            uint32_t f[N][8], amax = 0;
+            float sc[N];
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                sc[i] = __shfl_sync(0xffffffffu, v ? vs : ks, g * kKv8Block + r0 + i * RPW);
+                to_f16<FMT>(w[g][v][i].x, f[i][0], f[i][1]);
+                to_f16<FMT>(w[g][v][i].y, f[i][2], f[i][3]);
+                to_f16<FMT>(w[g][v][i].z, f[i][4], f[i][5]);
+                to_f16<FMT>(w[g][v][i].w, f[i][6], f[i][7]);
+                uint32_t m = 0;  // magnitudes, ordered as their bits
+#pragma unroll
+                for (int q = 0; q < 8; ++q) m = __vmaxu2(m, f[i][q] & 0x7fff7fffu);
+                const float top = __half2float(__ushort_as_half((unsigned short)max(m & 0xffffu, m >> 16))) * sc[i];
+                amax = max(amax, __float_as_uint(top) & 0x7fffffffu);
+            }
+            const float s = scale_for<FMT>(warp_umax(amax));
+            const bool nan = s != s;
+            const float inv = nan ? 0.0f : inverse(s);
+            if (lane == 0) (v ? a.dst.v_scale : a.dst.k_scale)[tile * kKv8Blocks + first % kKv8Page / kKv8Block] = s;
+            uint8_t* dst = static_cast<uint8_t*>(v ? a.dst.v : a.dst.k) + (tile * kKv8Page + first % kKv8Page) * D + c;
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int r = r0 + i * RPW;
+                // the ratio can pass f16's range where every code is small (2^17 for e4m3): then in two steps
+                float ratio = nan ? 0.0f : sc[i] * inv;
+                if (__any_sync(0xffffffffu, ratio > 16384.0f)) {
+                    const float part = fminf(ratio, 16384.0f);
+                    ratio = part > 0.0f ? fminf(ratio / part, 16384.0f) : 0.0f;
+                    const uint32_t p = __half_as_ushort(__float2half_rn(part)) * 0x10001u;
+#pragma unroll
+                    for (int q = 0; q < 8; ++q) f[i][q] = mul_f16(f[i][q], p);
+                }
+                const uint32_t p = __half_as_ushort(__float2half_rn(ratio)) * 0x10001u;
+#pragma unroll
+                for (int q = 0; q < 8; ++q) f[i][q] = mul_f16(f[i][q], p);
+                if (first + r < keep)
+                    *reinterpret_cast<uint4*>(dst + r * D) = make_uint4(from_f16<FMT>(f[i][0], f[i][1]), from_f16<FMT>(f[i][2], f[i][3]),
+                                                                        from_f16<FMT>(f[i][4], f[i][5]), from_f16<FMT>(f[i][6], f[i][7]));
+            }
+        }
     }
 }
 
@@ -321,9 +481,20 @@ struct AppendLaunch {
     cudaStream_t s;
     template <int FMT, int D>
     cudaError_t run() {
-        const int64_t units = (int64_t)a.kv.n_seqs * a.blocks * a.kv.kv_heads * 2;
-        kv8_append_kernel<FMT, D><<<blocks_of(units, 8), 256, 0, s>>>(a);
-        return cudaGetLastError();
+        const dim3 grid(blocks_of((int64_t)a.blocks * a.kv.kv_heads, 8), a.kv.n_seqs);
+        if (a.k.dtype == LASTRO_DTYPE_F32) return kv8_launch<kv8_append_kernel<FMT, D, true>>(grid, 256, 0, 1, s, a);
+        return kv8_launch<kv8_append_kernel<FMT, D, false>>(grid, 256, 0, 1, s, a);
+    }
+};
+
+struct ReadLaunch {
+    const Kv8ReadArgs& a;
+    cudaStream_t s;
+    template <int FMT, int D>
+    cudaError_t run() {
+        const dim3 grid(blocks_of(a.n, 8 * kReadSlots), a.kv.n_seqs);
+        if (a.f32) return kv8_launch<kv8_read_kernel<FMT, D, true>>(grid, 256, 0, 1, s, a);
+        return kv8_launch<kv8_read_kernel<FMT, D, false>>(grid, 256, 0, 1, s, a);
     }
 };
 
@@ -332,10 +503,16 @@ struct EvictLaunch {
     cudaStream_t s;
     template <int FMT, int D>
     cudaError_t run() {
-        kv8_select_kernel<<<dim3(a.src.kv_heads, a.src.n_seqs), kSelThreads, 0, s>>>(a);
-        const int64_t units = (int64_t)a.src.n_seqs * a.src.kv_heads * ((a.budget + kKv8Block - 1) / kKv8Block) * 2;
-        if (units) kv8_gather_kernel<FMT, D><<<blocks_of(units, 8), 256, 0, s>>>(a);
-        return cudaGetLastError();
+        // a cluster where one CTA's shared memory might not hold the keys
+        const int64_t slots = (int64_t)a.src.max_pages * kKv8Page;
+        const int cl = slots > kSelSlots ? 8 : 1;
+        const size_t smem = ((size_t)min((slots + cl - 1) / cl + 3, (int64_t)kSelSlots) + (cl > 1 ? 3 : 1) * kSelBins) * sizeof(uint32_t);
+        const dim3 grid(cl, a.src.kv_heads, a.src.n_seqs);
+        const cudaError_t e = cl > 1 ? kv8_launch<kv8_select_kernel<8>>(grid, 1024, smem, 8, s, a)
+                                     : kv8_launch<kv8_select_kernel<1>>(grid, 512, smem, 1, s, a);
+        if (e != cudaSuccess) return e;
+        const dim3 blocks(blocks_of(a.budget, 8 * 32), a.src.kv_heads, a.src.n_seqs);
+        return kv8_launch<kv8_gather_kernel<FMT, D>>(blocks, 256, 0, 1, s, a);
     }
 };
 
@@ -343,15 +520,6 @@ struct EvictLaunch {
 
 cudaError_t launch_kv8_append(const Kv8AppendArgs& a, cudaStream_t s) { return kv8_by_shape(a.kv, AppendLaunch{a, s}); }
 cudaError_t launch_kv8_evict(const Kv8EvictArgs& a, cudaStream_t s) { return kv8_by_shape(a.src, EvictLaunch{a, s}); }
-
-cudaError_t launch_kv8_read(const Kv8ReadArgs& a, cudaStream_t s) {
-    const int64_t total = (int64_t)a.kv.n_seqs * a.n * a.kv.kv_heads * (a.kv.head_dim / 8);
-    const unsigned int grid = (unsigned int)min((int64_t)148 * 16, (total + 255) / 256);
-    if (a.kv.format == E4M3)
-        (a.f32 ? kv8_read_kernel<E4M3, true> : kv8_read_kernel<E4M3, false>)<<<grid, 256, 0, s>>>(a);
-    else
-        (a.f32 ? kv8_read_kernel<INT8, true> : kv8_read_kernel<INT8, false>)<<<grid, 256, 0, s>>>(a);
-    return cudaGetLastError();
-}
+cudaError_t launch_kv8_read(const Kv8ReadArgs& a, cudaStream_t s) { return kv8_by_shape(a.kv, ReadLaunch{a, s}); }
 
 }  // namespace lastro

@@ -3,6 +3,8 @@
 
 #include <cuda_fp8.h>
 
+#include <atomic>
+
 #include "common.cuh"
 #include "kv8.h"
 
@@ -55,15 +57,19 @@ LDEV float scale_for(uint32_t amax) {
 // 1 / s of a power of two s = 2^e, -126 <= e <= 122: exact
 LDEV float inverse(float s) { return __uint_as_float((254u << 23) - (__float_as_uint(s) & 0x7f800000u)); }
 
+// the codes of four values times a power of two
 template <int FMT>
-LDEV uint32_t encode4(float a, float b, float c, float d) {
+LDEV uint32_t encode4(float a, float b, float c, float d, float inv) {
     if (FMT == E4M3) {
-        const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
-        const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
+        const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a * inv, b * inv), __NV_SATFINITE, __NV_E4M3);
+        const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c * inv, d * inv), __NV_SATFINITE, __NV_E4M3);
         return lo | (hi << 16);
     }
-    return (uint32_t)(__float2int_rn(a) & 0xff) | (uint32_t)(__float2int_rn(b) & 0xff) << 8 |
-           (uint32_t)(__float2int_rn(c) & 0xff) << 16 | (uint32_t)(__float2int_rn(d) & 0xff) << 24;
+    // 1.5 * 2^23 + x rounds x to a whole number, whose low byte is the sum's (the product is exact)
+    const float big = 12582912.0f;
+    const uint32_t p = __float_as_uint(fmaf(a, inv, big)), q = __float_as_uint(fmaf(b, inv, big));
+    const uint32_t r = __float_as_uint(fmaf(c, inv, big)), t = __float_as_uint(fmaf(d, inv, big));
+    return __byte_perm(__byte_perm(p, q, 0x40), __byte_perm(r, t, 0x40), 0x5410);
 }
 
 template <int FMT>
@@ -78,29 +84,48 @@ LDEV void decode4(uint32_t w, float (&v)[4]) {
     }
 }
 
-// 8 consecutive values of an activation row; `vec`: every such group is 16-byte aligned
+// 8 consecutive values of an activation row as they are stored; `vec`: every such group is 16-byte aligned
 template <bool F32>
-LDEV void load8(const lastro_rows& r, int64_t at, bool vec, float (&v)[8]) {
-    if (F32) {
-        const float* p = static_cast<const float*>(r.ptr) + at;
+struct Raw8 {
+    uint32_t w[F32 ? 8 : 4];
+
+    LDEV void load(const lastro_rows& r, int64_t at, bool vec) {
+        const char* p = static_cast<const char*>(r.ptr) + at * (F32 ? 4 : 2);
         if (vec) {
-            const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
-            v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-        } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = __ldg(p + i);
-        }
-    } else {
-        const uint16_t* p = static_cast<const uint16_t*>(r.ptr) + at;
-        if (vec) {
-            const uint4 a = __ldg(reinterpret_cast<const uint4*>(p));
-            v[0] = bf_lo(a.x), v[1] = bf_hi(a.x), v[2] = bf_lo(a.y), v[3] = bf_hi(a.y);
-            v[4] = bf_lo(a.z), v[5] = bf_hi(a.z), v[6] = bf_lo(a.w), v[7] = bf_hi(a.w);
-        } else {
+            for (int i = 0; i < (F32 ? 2 : 1); ++i) {
+                const uint4 v = __ldg(reinterpret_cast<const uint4*>(p) + i);
+                w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
+            }
+        } else if (F32) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = __uint_as_float((uint32_t)__ldg(p + i) << 16);
+            for (int i = 0; i < (F32 ? 8 : 4); ++i) w[i] = __ldg(reinterpret_cast<const uint32_t*>(p) + i);
+        } else {
+            const uint16_t* q = reinterpret_cast<const uint16_t*>(p);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = __ldg(q + 2 * i) | (uint32_t)__ldg(q + 2 * i + 1) << 16;
         }
     }
+    LDEV void zero() {
+#pragma unroll
+        for (int i = 0; i < (F32 ? 8 : 4); ++i) w[i] = 0;
+    }
+    // magnitudes' bits so far: f32 bits, or two bf16 side by side
+    LDEV void widest(uint32_t& m) const {
+#pragma unroll
+        for (int i = 0; i < (F32 ? 8 : 4); ++i) m = F32 ? max(m, w[i] & 0x7fffffffu) : __vmaxu2(m, w[i] & 0x7fff7fffu);
+    }
+    LDEV static uint32_t f32_bits(uint32_t m) { return F32 ? m : max(m << 16, m & 0xffff0000u); }
+    LDEV void values(float (&v)[8]) const {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = F32 ? __uint_as_float(w[F32 ? i : 0]) : i & 1 ? bf_hi(w[F32 ? 0 : i / 2]) : bf_lo(w[F32 ? 0 : i / 2]);
+    }
+};
+
+LDEV uint32_t two_bf16(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
 }
 
 LDEV bool vec_rows(const lastro_rows& r) {
@@ -108,7 +133,41 @@ LDEV bool vec_rows(const lastro_rows& r) {
     return ((reinterpret_cast<uintptr_t>(r.ptr) | (uintptr_t)(r.row_stride * e) | (uintptr_t)(r.head_stride * e)) & 15) == 0;
 }
 
+// row r of a KV head's query rows: which query, for `group` heads a query (single-token calls need no division)
+LDEV int query_of(int r, int group) { return r < group ? 0 : r / group; }
+
 LDEV uint32_t warp_umax(uint32_t v) { return __reduce_max_sync(0xffffffffu, v); }
+
+// programmatic launch: the kernel's CTAs are placed while the stream's previous kernel drains and wait for its end before
+// they touch memory.  The shared memory limit of a kernel is raised once on each device.
+template <auto KERNEL, typename A>
+cudaError_t kv8_launch(dim3 grid, int threads, size_t smem, int cluster, cudaStream_t s, const A& a) {
+    if (smem > 48 * 1024) {
+        static std::atomic<size_t> limit[64];
+        int dev = 0;
+        cudaError_t e = cudaGetDevice(&dev);
+        if (e != cudaSuccess) return e;
+        if (dev >= 64 || limit[dev].load(std::memory_order_relaxed) < smem) {
+            e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+            if (e != cudaSuccess) return e;
+            if (dev < 64) limit[dev].store(smem, std::memory_order_relaxed);
+        }
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = threads;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, KERNEL, a);
+}
 
 template <typename F>
 cudaError_t kv8_by_shape(const lastro_kv8& kv, F f) {

@@ -200,60 +200,65 @@ LDEV void find_part(int* room, int n_seqs, Work work, Part part, Note note, int&
 // rows take a second term.  The factor is positive (a negative scale goes into the operand), so that the largest product
 // is the largest score.
 template <int D, int E, bool F32>
+struct QRaw {  // the rows as they are stored: loads on their way while other work goes on
+    Raw8<F32> x[E][D / 32];
+
+    LDEV void fetch(const Kv8AttendArgs& a, const Seq& s, int h, int row0, bool vec) {
+        const int lane = threadIdx.x & 31, gq = lane >> 2, c = lane & 3;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const int r = row0 + gq + 8 * e, i = query_of(r, a.group);
+            const bool there = r < s.n * a.group;
+            const int64_t at = (int64_t)(s.first + i) * a.q.row_stride + (int64_t)(h * a.group + r - i * a.group) * a.q.head_stride + 16 * c;
+#pragma unroll
+            for (int k = 0; k < D / 32; ++k)
+                if (there)
+                    x[e][k].load(a.q, at + k / 2 * 64 + k % 2 * 8, vec);
+                else
+                    x[e][k].zero();
+        }
+    }
+};
+
+template <int D, int E, bool F32>
 struct QFrag {
     static constexpr int KS = D / 16;
     uint32_t hi[KS][2 * E], lo[F32 ? KS : 1][2 * E];  // [k step][k half, row half]
     float factor[E];
 
-    LDEV void load(const Kv8AttendArgs& a, const Seq& s, int h, int row0, bool vec) {
-        const int lane = threadIdx.x & 31, gq = lane >> 2, c = lane & 3;
+    LDEV void convert(const QRaw<D, E, F32>& raw, float scale) {
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            const int r = row0 + gq + 8 * e;
-            float x[D / 64][16];
-            uint32_t amax = 0;
+            uint32_t m = 0;
 #pragma unroll
-            for (int hf = 0; hf < D / 64; ++hf) {
-                if (r < s.n * a.group) {
-                    const int i = r / a.group;
-                    const int64_t at = (int64_t)(s.first + i) * a.q.row_stride +
-                                       (int64_t)(h * a.group + r - i * a.group) * a.q.head_stride + hf * 64 + 16 * c;
-                    float (&u)[8] = *reinterpret_cast<float (*)[8]>(&x[hf][0]);
-                    float (&w)[8] = *reinterpret_cast<float (*)[8]>(&x[hf][8]);
-                    load8<F32>(a.q, at, vec, u);
-                    load8<F32>(a.q, at + 8, vec, w);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) x[hf][i] = 0.0f;
-                }
-#pragma unroll
-                for (int i = 0; i < 16; ++i) amax = max(amax, __float_as_uint(x[hf][i]) & 0x7fffffffu);
-            }
+            for (int k = 0; k < D / 32; ++k) raw.x[e][k].widest(m);
+            uint32_t amax = Raw8<F32>::f32_bits(m);
             amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
             amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
             const int k = min(126, 141 - (int)(amax >> 23));  // 14 - exponent
             const bool finite = amax < 0x7f800000u;
-            const float up = finite ? copysignf(__uint_as_float((uint32_t)(k + 127) << 23), a.scale) : 0.0f;
-            factor[e] = finite ? fabsf(a.scale) * 1.44269504088896340736f * __uint_as_float((uint32_t)(127 - k) << 23)
+            const float up = copysignf(__uint_as_float((uint32_t)(k + 127) << 23), scale);
+            factor[e] = finite ? fabsf(scale) * 1.44269504088896340736f * __uint_as_float((uint32_t)(127 - k) << 23)
                                : __uint_as_float(0x7fc00000u);
 #pragma unroll
-            for (int hf = 0; hf < D / 64; ++hf)
+            for (int i = 0; i < D / 32; ++i) {
+                float v[8];
+                raw.x[e][i].values(v);
 #pragma unroll
-                for (int q = 0; q < 4; ++q)
-#pragma unroll
-                    for (int w = 0; w < 2; ++w) {
-                        const float u = finite ? x[hf][4 * q + 2 * w] * up : 0.0f;
-                        const float v = finite ? x[hf][4 * q + 2 * w + 1] * up : 0.0f;
-                        hi[hf * 4 + q][w * E + e] = pack_f16(u, v);
-                        if (F32) lo[F32 ? hf * 4 + q : 0][w * E + e] = rest_f16(hi[hf * 4 + q][w * E + e], u, v);
-                    }
+                for (int j = 0; j < 4; ++j) {
+                    const float u = finite ? v[2 * j] * up : 0.0f, w = finite ? v[2 * j + 1] * up : 0.0f;
+                    uint32_t& t = hi[2 * i + j / 2][(j & 1) * E + e];
+                    t = pack_f16(u, w);
+                    if (F32) lo[F32 ? 2 * i + j / 2 : 0][(j & 1) * E + e] = rest_f16(t, u, w);
+                }
+            }
         }
     }
 };
 
 // slots that row r of the sequence sees
 LDEV int visible(const Kv8AttendArgs& a, const Seq& s, int r) {
-    return s.len - s.n + min(r, s.n * a.group - 1) / a.group + 1;
+    return s.len - s.n + query_of(min(r, s.n * a.group - 1), a.group) + 1;
 }
 
 // the codes of slot row `row` that this lane feeds to the score product: 16 bytes of every 64
@@ -327,8 +332,8 @@ struct WarpRows {
         return v;
     }
 
-    LDEV void begin(const Kv8AttendArgs& a, const Seq& s, int h, int row0, bool vec) {
-        q.load(a, s, h, row0, vec);
+    LDEV void begin(const Kv8AttendArgs& a, const Seq& s, int row0, const QRaw<D, E, F32>& raw) {
+        q.convert(raw, a.scale);
 #pragma unroll
         for (int j = 0; j < (FEW ? D / 16 : D / 8); ++j)
 #pragma unroll
@@ -389,13 +394,20 @@ struct WarpRows {
         for (int b = 0; b < NB; ++b) {
             scores(sk + b * 16 * D, s[b]);
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                fk[b][e] = fac[e] * ks[b];
-                if (!WHOLE)
+            for (int e = 0; e < 2; ++e) fk[b][e] = fac[e] * ks[b];
+        }
+        uint32_t hidden = 0;  // of this lane's scores, those whose row does not see the slot
+        if (!WHOLE) {
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
 #pragma unroll
                     for (int k = 0; k < NT; ++k)
-                        if (t0 + b * 16 + slot(k) >= vis[e]) s[b][e][k] = -INFINITY;
-            }
+                        if (t0 + b * 16 + slot(k) >= vis[e]) {
+                            s[b][e][k] = -INFINITY;
+                            hidden |= 1u << ((b * 2 + e) * NT + k);
+                        }
         }
         if (FEW && keep) {
 #pragma unroll
@@ -406,7 +418,7 @@ struct WarpRows {
 #pragma unroll
                         for (int k = 0; k < NT; ++k)
                             keep[row_of(e) * NB * 16 + b * 16 + slot(k)] =
-                                !WHOLE && s[b][e][k] == -INFINITY ? -INFINITY : s[b][e][k] * fk[b][e];
+                                hidden >> ((b * 2 + e) * NT + k) & 1 ? -INFINITY : s[b][e][k] * fk[b][e];
         }
         float Mn[2], Rn[2];
         bool moved = false;
@@ -442,24 +454,40 @@ struct WarpRows {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) o[j][i] *= f[FEW ? i & 1 : i >> 1];
         }
+        // s becomes the weights: first 2^(score - M), which l sums, then what multiplies the V codes
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+#pragma unroll
+                for (int k = 0; k < NT; ++k) s[b][e][k] = ex2(fmaf(s[b][e][k], fk[b][e], -M[e]));
+        if (!WHOLE) {
+#pragma unroll
+            for (int i = 0; i < NB * 2 * NT; ++i)
+                if (hidden >> i & 1) s[i / (2 * NT)][i / NT % 2][i % NT] = 0.0f;
+        }
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                // at most 2^14 / (the block's largest weight); kept finite where that weight is below the smallest f32
+                const float f = min_nan(vs[b] * g[e], 1.7e38f);
+#pragma unroll
+                for (int k = 0; k < NT; ++k) {
+                    l[e] += s[b][e][k];
+                    s[b][e][k] *= f;
+                }
+            }
+        if (!WHOLE) {  // a NaN scale must not reach the rows that do not see the slot
+#pragma unroll
+            for (int i = 0; i < NB * 2 * NT; ++i)
+                if (hidden >> i & 1) s[i / (2 * NT)][i / NT % 2][i % NT] = 0.0f;
+        }
         // the weights as product operands, first and second terms
         uint32_t pa[NB][FEW ? 2 : 4], pb[F32 ? NB : 1][FEW ? 2 : 4];
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
-            float w[2][NT];
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                // at most 2^14 / (the block's largest p); kept finite where that p is below the smallest f32
-                const float f = min_nan(vs[b] * g[e], 1.7e38f);
-#pragma unroll
-                for (int k = 0; k < NT; ++k) {
-                    float p = ex2(fmaf(s[b][e][k], fk[b][e], -M[e]));
-                    w[e][k] = p * f;
-                    // slots the row does not see; a NaN scale of theirs must not reach it
-                    if (!WHOLE && s[b][e][k] == -INFINITY) p = w[e][k] = 0.0f;
-                    l[e] += p;
-                }
-            }
+            const float(&w)[2][NT] = s[b];
             if constexpr (FEW) {
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
@@ -538,7 +566,7 @@ struct WarpRows {
 
     // row e of this lane to the output: the unit is complete
     LDEV void store(const Kv8AttendArgs& a, const Seq& s, int h, int r, int e, bool vec) const {
-        const int i = r / a.group, t = s.first + i, hq = h * a.group + r - i * a.group;
+        const int i = query_of(r, a.group), t = s.first + i, hq = h * a.group + r - i * a.group;
         const float inv = l[e] == 0.0f ? 0.0f : 1.0f / l[e], up = pow2i(R[e] - 14.0f - M[e]);
 #pragma unroll
         for (int hf = 0; hf < D / 64; ++hf) {
@@ -560,7 +588,7 @@ struct WarpRows {
                 uint16_t* dst = static_cast<uint16_t*>(a.out.ptr) + at;
                 uint32_t w[RUN / 2];
 #pragma unroll
-                for (int k = 0; k < RUN / 2; ++k) w[k] = pack_bf16(f32_to_bf16_rne(v[2 * k]), f32_to_bf16_rne(v[2 * k + 1]));
+                for (int k = 0; k < RUN / 2; ++k) w[k] = two_bf16(v[2 * k], v[2 * k + 1]);
                 if (vec) {
 #pragma unroll
                     for (int k = 0; k < RUN / 8; ++k)
@@ -626,7 +654,7 @@ LDEV void add_parts(int n, At at, float (&o)[D / 32], float& M, float& R, float&
 template <int D, bool F32>
 LDEV void store_merged(const Kv8AttendArgs& a, int first, int h, int r, const float (&o)[D / 32], float M, float R, float l) {
     constexpr int V = D / 32;
-    const int lane = threadIdx.x & 31, i = r / a.group, t = first + i, hq = h * a.group + r - i * a.group;
+    const int lane = threadIdx.x & 31, i = query_of(r, a.group), t = first + i, hq = h * a.group + r - i * a.group;
     const float inv = l == 0.0f ? 0.0f : 1.0f / l, up = pow2i(R - 14.0f - M);
     const int64_t at = (int64_t)t * a.out.row_stride + (int64_t)hq * a.out.head_stride + lane * V;
 #pragma unroll
@@ -766,22 +794,25 @@ __global__ void __launch_bounds__(Shape<D, FEW, RW>::THREADS, 1) kv8_attend_kern
             advance(iss);
             if (iss.c == 0) limit();
         };
-        limit();
-        if (wrow == 0)
-            for (int i = 0; i < min(ST, count); ++i) issue(i);
-
+        // the rows' loads go out first: they and the page numbers are on their way together
         const bool vq = vec_rows(a.q);
         WarpRows<FMT, D, FEW, F32> rows;
+        QRaw<D, FEW ? 1 : 2, F32> raw;
         int row0 = 0, vmin = 0, nrows = 0;  // the warp's first row of the unit, what it sees, and the rows from there on
         bool from0 = false;                 // the unit began in this part
+        auto fetch_unit = [&]() { raw.fetch(a, cur.s, cur.h, cur.tile * TILE + wrow * SH::ROWS, vq); };
         auto begin_unit = [&]() {
             row0 = cur.tile * TILE + wrow * SH::ROWS;
             nrows = cur.s.n * a.group - row0;
             from0 = cur.c == 0;
             if (nrows <= 0) return;
             vmin = visible(a, cur.s, row0);
-            rows.begin(a, cur.s, cur.h, row0, vq);
+            rows.begin(a, cur.s, row0, raw);
         };
+        fetch_unit();
+        limit();
+        if (wrow == 0)
+            for (int i = 0; i < min(ST, count); ++i) issue(i);
         begin_unit();
 
         bool alive = true;
@@ -810,6 +841,11 @@ __global__ void __launch_bounds__(Shape<D, FEW, RW>::THREADS, 1) kv8_attend_kern
             }
             const bool last = cur.c == cur.s.chunks - 1;
             if (last || it == count - 1) {
+                const Cursor was = cur;
+                if (it + 1 < count) {
+                    advance(cur);
+                    fetch_unit();
+                }
                 if (nrows > 0) {
                     rows.finish();
 #pragma unroll
@@ -817,7 +853,7 @@ __global__ void __launch_bounds__(Shape<D, FEW, RW>::THREADS, 1) kv8_attend_kern
                         const int r = rows.row_of(e);
                         if (r >= nrows) continue;
                         if (last && from0)
-                            rows.store(a, cur.s, cur.h, row0 + r, e, vo);
+                            rows.store(a, was.s, was.h, row0 + r, e, vo);
                         else if (RW > 1)
                             rows.leave(a.part + (((int64_t)group * 2 + from0) * TILE + wrow * SH::ROWS + r) * SH::PART, e);
                         else if (from0)  // its ring is empty by now
@@ -829,14 +865,11 @@ __global__ void __launch_bounds__(Shape<D, FEW, RW>::THREADS, 1) kv8_attend_kern
                 if (RW == 1 && lane == 0 && !(last && from0)) {
                     Ends& x = ends[warp];
                     if (from0)
-                        x.tail = true, x.th = cur.h, x.tt = cur.tile, x.tn = cur.s.n, x.tfirst = cur.s.first;
+                        x.tail = true, x.th = was.h, x.tt = was.tile, x.tn = was.s.n, x.tfirst = was.s.first;
                     else
-                        x.mid = true, x.closes = last, x.hh = cur.h, x.ht = cur.tile, x.hn = cur.s.n, x.hfirst = cur.s.first;
+                        x.mid = true, x.closes = last, x.hh = was.h, x.ht = was.tile, x.hn = was.s.n, x.hfirst = was.s.first;
                 }
-                if (it + 1 < count) {
-                    advance(cur);
-                    begin_unit();
-                }
+                if (it + 1 < count) begin_unit();
             } else {
                 ++cur.c;
             }
@@ -849,12 +882,18 @@ __global__ void __launch_bounds__(Shape<D, FEW, RW>::THREADS, 1) kv8_attend_kern
     // the units that the warps of this CTA cut, row by row: to the output when all of one is here, else to this share's
     // slots.  A run begins with the unit the share begins inside of (which < 0) or with the one warp `which` left open.
     __syncthreads();
+    const Ends mine = ends[lane & (SH::WARPS - 1)];
+    const unsigned low = (1u << SH::WARPS) - 1, mids = __ballot_sync(0xffffffffu, mine.mid) & low;
+    const unsigned tails = __ballot_sync(0xffffffffu, mine.tail) & low, closes = __ballot_sync(0xffffffffu, mine.mid && mine.closes) & low;
     int task = 0;  // rows of the runs, dealt to the warps
-    for (int which = -1; which < SH::WARPS; ++which) {
-        if (which < 0 ? !ends[0].mid : !ends[which].tail) continue;
-        int n = which < 0 ? 0 : 1;  // parts before warp which + 1's
-        bool closed = false;
-        for (int j = which + 1; j < SH::WARPS && ends[j].mid && !closed; ++j, ++n) closed = ends[j].closes;
+    for (unsigned starts = tails << 1 | (mids & 1); starts; starts &= starts - 1) {
+        const int which = __ffs(starts) - 2;
+        // warps which + 1, ... that began inside it, up to the one that closes it
+        const unsigned after = mids >> (which + 1), ended = closes >> (which + 1);
+        int n = __ffs(~after) - 1;
+        const bool closed = (ended & ((1u << n) - 1)) != 0;
+        if (closed) n = __ffs(ended);
+        n += which >= 0;
         const Ends& x = ends[max(which, 0)];
         const int h = which < 0 ? x.hh : x.th, tile = which < 0 ? x.ht : x.tt, row0 = which < 0 ? x.hfirst : x.tfirst;
         const int first = max(which, 0), nrows = min(SH::ROWS, (which < 0 ? x.hn : x.tn) * a.group - tile * TILE);
@@ -993,7 +1032,9 @@ __global__ void __launch_bounds__(kThreads) kv8_mass_kernel(const __grid_constan
             if (warp < nt) {
                 const int row0 = (tb + warp) * 16;
                 QFrag<D, 2, F32> q;
-                q.load(a, s, h, row0, vq);
+                QRaw<D, 2, F32> raw;
+                raw.fetch(a, s, h, row0, vq);
+                q.convert(raw, a.scale);
 #pragma unroll
                 for (int k = 0; k < KS; ++k) {
                     qs[(warp * KS + k) * 32 + lane] = make_uint4(q.hi[k][0], q.hi[k][1], q.hi[k][2], q.hi[k][3]);
@@ -1101,25 +1142,6 @@ int sm_count() {
     return n;
 }
 
-template <typename K>
-cudaError_t launch(K kernel, dim3 grid, int threads, size_t smem, cudaStream_t s, const Kv8AttendArgs& a) {
-    if (smem > 48 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-        if (e != cudaSuccess) return e;
-    }
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = threads;
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = s;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, a);
-}
-
 struct AttendLaunch {
     Kv8AttendArgs a;
     cudaStream_t s;
@@ -1128,17 +1150,17 @@ struct AttendLaunch {
     cudaError_t go() {
         using SH = Shape<D, FEW, RW>;
         a.shares = sm_count() * (RW == 1 ? 1 : SH::GROUPS);
-        cudaError_t e = launch(kv8_attend_kernel<FMT, D, FEW, RW, F32>, dim3(sm_count()), SH::THREADS, SH::SMEM, s, a);
+        cudaError_t e = kv8_launch<kv8_attend_kernel<FMT, D, FEW, RW, F32>>(dim3(sm_count()), SH::THREADS, SH::SMEM, 1, s, a);
         if (e != cudaSuccess) return e;
         const int64_t rows = (int64_t)a.max_new * a.heads;
         const dim3 grid((unsigned)min((int64_t)1024, (rows + kWarps - 1) / kWarps), a.kv.n_seqs);
-        e = launch(kv8_merge_kernel<D, FEW, RW, F32>, grid, kThreads, 0, s, a);
+        e = kv8_launch<kv8_merge_kernel<D, FEW, RW, F32>>(grid, kThreads, 0, 1, s, a);
         if (e != cudaSuccess || !a.mass_out) return e;
         if (a.scores) {
             const dim3 blocks(min(64, (a.kv.max_pages * kKv8Page + 511) / 512), a.kv.kv_heads, a.kv.n_seqs);
-            return launch(kv8_weights_kernel<D>, blocks, 128, 0, s, a);
+            return kv8_launch<kv8_weights_kernel<D>>(blocks, 128, 0, 1, s, a);
         }
-        return launch(kv8_mass_kernel<FMT, D, F32>, dim3(2 * sm_count()), kThreads, mass_smem<D, F32>(), s, a);
+        return kv8_launch<kv8_mass_kernel<FMT, D, F32>>(dim3(2 * sm_count()), kThreads, mass_smem<D, F32>(), 1, s, a);
     }
     template <int FMT, int D, bool FEW, int RW>
     cudaError_t by_type() {

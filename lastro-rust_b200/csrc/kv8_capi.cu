@@ -67,6 +67,7 @@ extern "C" int lastro_kv8_append(lastro_ctx* ctx, const lastro_kv8* kv, const in
     KV8_TRY(check_rows(ctx, v, "kv8_append: v"));
     if (!lens || !new_off || !lens_out) return set_err(ctx, LASTRO_E_ARG, "kv8_append: null lens, new_off or lens_out");
     if (lens == lens_out) return set_err(ctx, LASTRO_E_ARG, "kv8_append: lens_out must not be lens");
+    if (k->dtype != v->dtype) return set_err(ctx, LASTRO_E_ARG, "kv8_append: k and v of different dtypes");
     if (max_new < 0) return set_err(ctx, LASTRO_E_ARG, "kv8_append: max_new %d", max_new);
     if (mass && mass_stride < 1) return set_err(ctx, LASTRO_E_ARG, "kv8_append: mass_stride %lld", (long long)mass_stride);
     Kv8AppendArgs a{};

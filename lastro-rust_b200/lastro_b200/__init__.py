@@ -800,6 +800,9 @@ class GpuBatch:
 _ROW_DTYPES = {"torch.bfloat16": DTYPE_BF16, "torch.float32": DTYPE_F32, "bf16": DTYPE_BF16, "f32": DTYPE_F32}
 
 
+_row_dtypes = {}  # the same by the dtype objects met so far
+
+
 def _dev(x):
     """A device address: an int, None, or anything with data_ptr() (a torch tensor)."""
     return x if x is None or isinstance(x, int) else x.data_ptr()
@@ -807,11 +810,13 @@ def _dev(x):
 
 def rows_of(t) -> Rows:
     """The lastro_rows of a torch-like device tensor [rows, heads, head_dim], bf16 or f32, the last axis dense."""
-    rows, head = t.stride()[:2]
-    dtype = _ROW_DTYPES.get(str(t.dtype))
-    if dtype is None or t.ndim != 3 or t.stride(2) != 1:
-        raise LastroError(E_ARG, f"rows: {tuple(t.shape)} {t.dtype} with strides {t.stride()} (bf16 or f32, last axis dense)")
-    return Rows(t.data_ptr(), dtype, t.shape[0], rows, head)
+    strides = t.stride()
+    dtype = _row_dtypes.get(t.dtype)
+    if dtype is None:
+        dtype = _row_dtypes[t.dtype] = _ROW_DTYPES.get(str(t.dtype), 0)
+    if not dtype or len(strides) != 3 or strides[2] != 1:
+        raise LastroError(E_ARG, f"rows: {tuple(t.shape)} {t.dtype} with strides {strides} (bf16 or f32, last axis dense)")
+    return Rows(t.data_ptr(), dtype, t.shape[0], strides[0], strides[1])
 
 
 class Kv8Cache:
@@ -831,17 +836,18 @@ class Kv8Cache:
         self.buffers = (k, v, k_scale, v_scale, page_table, status)  # tensors live as long as the cache
         self.desc = Kv8Desc(KV8_FORMATS[fmt], n_seqs, kv_heads, head_dim, num_pages, max_pages,
                             *(_dev(x) for x in self.buffers))
+        self._kv = C.byref(self.desc)
 
     def append(self, lens, new_off, max_new: int, k: Rows, v: Rows, lens_out, mass=None, mass_stride: int = 0):
         """Quantise rows [new_off[b], new_off[b + 1]) of k and v into slots lens[b].. of each sequence
         (lastro_kv8_append)."""
-        self.ctx.check(lib().lastro_kv8_append(self.ctx.h, self.desc, _dev(lens), _dev(new_off), max_new, k, v,
+        self.ctx.check(lib().lastro_kv8_append(self.ctx.h, self._kv, _dev(lens), _dev(new_off), max_new, k, v,
                                                _dev(lens_out), _dev(mass), mass_stride))
 
     def attend_workspace(self, heads: int, max_new: int, with_mass: bool) -> int:
         """Bytes of workspace attend() needs."""
         n = C.c_size_t()
-        self.ctx.check(lib().lastro_kv8_attend_workspace(self.ctx.h, self.desc, heads, max_new, int(with_mass),
+        self.ctx.check(lib().lastro_kv8_attend_workspace(self.ctx.h, self._kv, heads, max_new, int(with_mass),
                                                          C.byref(n)))
         return n.value
 
@@ -849,7 +855,7 @@ class Kv8Cache:
                workspace_bytes: int, mass_in=None, mass_out=None, mass_stride: int = 0):
         """out = softmax(scale * q k) v over the slots each query sees; mass_out = mass_in + the weights each slot
         received (lastro_kv8_attend)."""
-        self.ctx.check(lib().lastro_kv8_attend(self.ctx.h, self.desc, _dev(lens), _dev(q_off), max_new, heads, q, scale,
+        self.ctx.check(lib().lastro_kv8_attend(self.ctx.h, self._kv, _dev(lens), _dev(q_off), max_new, heads, q, scale,
                                                out, _dev(mass_in), _dev(mass_out), mass_stride, _dev(workspace),
                                                workspace_bytes))
 
@@ -857,12 +863,12 @@ class Kv8Cache:
               mass_out=None, mass_out_stride: int = 0):
         """Cut every sequence to `budget` slots by accumulated mass, its kept rows written to dst's pages
         (lastro_kv8_evict)."""
-        self.ctx.check(lib().lastro_kv8_evict(self.ctx.h, self.desc, dst.desc, _dev(lens), budget, recent, _dev(mass),
+        self.ctx.check(lib().lastro_kv8_evict(self.ctx.h, self._kv, dst._kv, _dev(lens), budget, recent, _dev(mass),
                                               mass_stride, _dev(kept), _dev(lens_out), _dev(mass_out), mass_out_stride))
 
     def read(self, lens, pos0, n: int, k_out, v_out, dtype: str):
         """The values of slots [pos0[b], pos0[b] + n) of every sequence as bf16 or f32 (lastro_kv8_read)."""
         if dtype not in ("bf16", "f32"):
             raise LastroError(E_ARG, f"dtype {dtype!r} (bf16 or f32)")
-        self.ctx.check(lib().lastro_kv8_read(self.ctx.h, self.desc, _dev(lens), _dev(pos0), n, _dev(k_out), _dev(v_out),
+        self.ctx.check(lib().lastro_kv8_read(self.ctx.h, self._kv, _dev(lens), _dev(pos0), n, _dev(k_out), _dev(v_out),
                                              _ROW_DTYPES[dtype]))
