@@ -78,6 +78,19 @@ LDEV uint32_t rest_f16(uint32_t packed, float lo, float hi) {
     return pack_f16(lo - f.x, hi - f.y);
 }
 
+// bulk_g2s for data read once: its lines leave L2 before others
+LDEV void bulk_g2s_once(void* dst, const void* src, uint32_t bytes, uint64_t* bar, uint64_t policy) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1], %2, [%3], %4;" ::"r"(
+                     smem_addr(dst)),
+                 "l"(src), "r"(bytes), "r"(smem_addr(bar)), "l"(policy)
+                 : "memory");
+}
+LDEV uint64_t read_once() {
+    uint64_t p;
+    asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(p));
+    return p;
+}
+
 LDEV void mbar_arrive(uint64_t* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
 }
@@ -88,24 +101,27 @@ LDEV int slot_of(int pair, int e, int j) { return j * 8 + e * 4 + (pair & 2) + (
 
 // ---- shapes -------------------------------------------------------------------------------------------------------------
 // How a call's units (one sequence, KV head and tile of query rows) are worked on: RW of a CTA's 8 warps side by side take
-// a tile of RW * ROWS rows and share the stages of one ring.  Few rows with 16 warps of half the chunk instead: 315 against
-// 267 us at 96 sequences of 8192 slots, 32 heads of 128 (the work around a chunk counts for more than the latency that
-// more warps hide).
+// a tile of RW * ROWS rows and share the stages of one ring.
+//   Few rows with 16 warps of half the chunk instead: 315 against 267 us at 96 sequences of 8192 slots, 32 heads of 128 (the
+//   work around a chunk counts for more than the latency that more warps hide).
+//   More than 16 rows in tiles of 16, 32, 64 or 128 rows (RW 1, 2, 4, 8): 39.6, 33.5, 39.4 and 40.6 us at 8 sequences of
+//   2048 slots with 32 queries of 24 heads, 28.2, 27.5, 27.4 and 33.8 with 16, 309, 317, 395 and 426 at 32 sequences of
+//   8192: two warps that share a stage halve its traffic, more of them wait on one another or have no rows.
 template <int D, bool FEW, int RW>
 struct Shape {
     static constexpr int WARPS = 8, THREADS = WARPS * 32, GROUPS = WARPS / RW;
     static constexpr int ROWS = FEW ? 8 : 16, TILE = RW * ROWS;     // query rows of a warp and of a unit
     static constexpr int CHUNK = 4096, TOK = CHUNK / D; // K (or V) codes and slots of a stage
     static constexpr int NB = TOK / kKv8Block, CPP = kKv8Page / TOK; // blocks of a chunk, chunks of a page
-    static constexpr int STAGES = FEW ? 3 : RW == 1 ? 2 : RW == 2 ? 6 : 8;
+    static constexpr int STAGES = FEW ? 3 : RW == 1 ? 2 : 6;
     static constexpr int PART = D + 4;  // floats of one row's partial result: its sums, then M, R and l
     static constexpr int BARS = RW == 1 ? 1 : 2;  // a warp on its own needs no barrier to hand stages back
     static constexpr size_t HEAD = RW == 1 ? (size_t)ROWS * PART * sizeof(float) : 0;
     static constexpr size_t SMEM = (size_t)GROUPS * (STAGES * (2 * CHUNK + 8 * sizeof(float) + BARS * 8 + 4) + HEAD);
 };
 
-// warps that share a unit: as many 16-row tiles as the largest has, up to 8; 0 stands for few rows
-int row_warps(int64_t rows) { return rows <= 8 ? 0 : rows <= 16 ? 1 : rows <= 32 ? 2 : rows <= 64 ? 4 : 8; }
+// the form for units of at most `rows` rows: 0 few rows, else the warps that share a unit
+int row_warps(int64_t rows) { return rows <= 8 ? 0 : rows <= 16 ? 1 : 2; }
 
 // ---- the list of work -------------------------------------------------------------------------------------------------
 // Every sequence with queries contributes kv_heads * row tiles * chunks items, chunks innermost; equal consecutive shares
@@ -759,6 +775,7 @@ __global__ void __launch_bounds__(Shape<D, FEW, RW>::THREADS, 1) kv8_attend_kern
             } while (x.s.tiles == 0);
         };
 
+        const uint64_t policy = FEW ? read_once() : 0;
         // page numbers ahead of the issuing cursor: lane i holds page pbase + i of sequence pb
         int pb = -1, pbase = 0, pnum = 0;
         int seen = 0;  // chunks of the issuing cursor's unit that any of its rows sees
@@ -783,8 +800,14 @@ __global__ void __launch_bounds__(Shape<D, FEW, RW>::THREADS, 1) kv8_attend_kern
                     const int64_t at = tile * kKv8Page * D + (int64_t)(iss.c % CPP) * SH::CHUNK;
                     unsigned char* dst = data + (size_t)st * STAGE;
                     mbar_expect_tx(full + st, STAGE + 32);
-                    bulk_g2s(dst, static_cast<const uint8_t*>(a.kv.k) + at, SH::CHUNK, full + st);
-                    bulk_g2s(dst + SH::CHUNK, static_cast<const uint8_t*>(a.kv.v) + at, SH::CHUNK, full + st);
+                    const uint8_t *k = static_cast<const uint8_t*>(a.kv.k) + at, *v = static_cast<const uint8_t*>(a.kv.v) + at;
+                    if (FEW) {  // read once, and the scores kept meanwhile stay in L2 for the weights
+                        bulk_g2s_once(dst, k, SH::CHUNK, full + st, policy);
+                        bulk_g2s_once(dst + SH::CHUNK, v, SH::CHUNK, full + st, policy);
+                    } else {
+                        bulk_g2s(dst, k, SH::CHUNK, full + st);
+                        bulk_g2s(dst + SH::CHUNK, v, SH::CHUNK, full + st);
+                    }
                     bulk_g2s(scales + st * 8, a.kv.k_scale + tile * kKv8Blocks, 16, full + st);
                     bulk_g2s(scales + st * 8 + 4, a.kv.v_scale + tile * kKv8Blocks, 16, full + st);
                 } else {
@@ -820,12 +843,14 @@ __global__ void __launch_bounds__(Shape<D, FEW, RW>::THREADS, 1) kv8_attend_kern
             const int st = it % ST, ph = (it / ST) & 1;
             alive = mbar_wait(full + st, ph, a.kv.status, LASTRO_KV8_BAD_WAIT);
             if (!alive) break;
-            if (nrows > 0 && there[st]) {
+            if (nrows > 0) {
                 const unsigned char* sk = data + (size_t)st * STAGE;
                 const float* sc = scales + st * 8 + (cur.c % CPP) * NB;
                 const int t0 = cur.c * TOK;
                 float* keep = FEW && a.scores ? a.scores + (int64_t)(beg + it) * a.score_rows * TOK : nullptr;
-                if (t0 + TOK <= vmin)
+                if (!there[st]) {
+                    for (int i = lane; keep && i < nrows * TOK; i += 32) keep[i] = -INFINITY;
+                } else if (t0 + TOK <= vmin)
                     rows.template consume<true, NB>(sk, sk + SH::CHUNK, sc, sc + 4, t0, cur.s.len, keep, nrows);
                 else
                     rows.template consume<false, NB>(sk, sk + SH::CHUNK, sc, sc + 4, t0, cur.s.len, keep, nrows);
@@ -944,24 +969,51 @@ __global__ void __launch_bounds__(kThreads) kv8_merge_kernel(const __grid_consta
 
 // ---- accumulated weights, from stored scores ------------------------------------------------------------------------------
 // With few query rows the pass over the cache also leaves its scores (4 bytes a row and slot, against d bytes of K), and
-// the weights are one elementwise pass over them: a thread takes four slots.
-template <int D>
+// the weights are one elementwise pass over them: a thread takes four slots.  The kernel merges the shares too: every CTA
+// needs the merged sums of its KV head's rows, and the head's first CTA their outputs.
+template <int D, bool F32>
 __global__ void __launch_bounds__(128) kv8_weights_kernel(const __grid_constant__ Kv8AttendArgs a) {
     using SH = Shape<D, true, 1>;
+    __shared__ float sums[SH::ROWS];
     pdl_wait();
     pdl_launch();
-    const int b = blockIdx.z, h = blockIdx.y, H = a.kv.kv_heads;
+    const int b = blockIdx.z, h = blockIdx.y, H = a.kv.kv_heads, lane = threadIdx.x & 31;
     const Seq s = seq_of<SH::TOK, SH::TILE>(a, b);
     const int base = a.offset[b] + h * s.chunks, rows = s.n * a.group;
-    float lse[8];
+    const int per = share_of(a.offset[a.kv.n_seqs], a.shares), g0 = rows ? base / per : 0, g1 = rows ? (base + s.chunks - 1) / per : 0;
+    if (blockIdx.x * 512 >= s.len && blockIdx.x > 0) return;
+    for (int r = threadIdx.x >> 5; r < rows; r += 4) {
+        if (g0 == g1) {
+            const int i = query_of(r, a.group);
+            if (lane == 0) sums[r] = __ldcg(a.lse + (int64_t)(s.first + i) * a.heads + h * a.group + r - i * a.group);
+            continue;
+        }
+        const auto part = [&](int g) { return a.part + (((int64_t)g * 2 + (g == g0)) * SH::TILE + r) * SH::PART; };
+        float o[D / 32] = {}, M = kFar, R = kFar, l = 0.0f;
+        for (int g = g0; g <= g1; g += 32) {
+            const int n = min(32, g1 + 1 - g);
+            if (blockIdx.x == 0) {
+                add_parts<D>(n, [&](int k) { return part(g + k); }, o, M, R, l);
+            } else {
+                const float4 m = lane < n ? *reinterpret_cast<const float4*>(part(g + lane) + D) : make_float4(kFar, kFar, 0.0f, 0.0f);
+                const float Mn = fmaxf(M, warp_max(m.x));
+                l = l * pow2i(M - Mn) + warp_sum(m.z * pow2i(m.x - Mn));
+                M = Mn;
+            }
+        }
+        if (blockIdx.x == 0) store_merged<D, F32>(a, s.first, h, r, o, M, R, l);
+        if (lane == 0) sums[r] = l == 0.0f ? INFINITY : M + log2f(l);
+    }
+    __syncthreads();
+    float lse[SH::ROWS];
 #pragma unroll
-    for (int r = 0; r < 8; ++r)
-        if (r < rows) lse[r] = __ldcg(a.lse + (int64_t)(s.first + r / a.group) * a.heads + h * a.group + r % a.group);
+    for (int r = 0; r < SH::ROWS; ++r)
+        if (r < rows) lse[r] = sums[r];
     const int64_t at = ((int64_t)b * H + h) * a.mass_stride;
     const bool vec = ((reinterpret_cast<uintptr_t>(a.mass_out + at) | reinterpret_cast<uintptr_t>(a.mass_in ? a.mass_in + at : nullptr)) & 15) == 0;
     for (int t = (blockIdx.x * 128 + threadIdx.x) * 4; t < s.len; t += gridDim.x * 512) {
         float sum[4] = {};
-        if (rows > 0 && page_of(a.kv, b, t) >= 0) {
+        if (rows > 0) {
             const float* src = a.scores + (int64_t)(base + t / SH::TOK) * a.score_rows * SH::TOK + t % SH::TOK;
 #pragma unroll
             for (int r = 0; r < 8; ++r)
@@ -1028,6 +1080,23 @@ __global__ void __launch_bounds__(kThreads) kv8_mass_kernel(const __grid_constan
         const int rows = s.n * a.group, tiles = s.tiles;
         for (int tb = 0; tb < max(1, tiles); tb += kMassTiles) {
             const int nt = min(kMassTiles, tiles - tb);
+            // a chunk's K codes as they are stored: the first is on its way while the rows are made ready
+            int page = -1;
+            uint32_t w[NB][2][KS];
+            float ks_next[NB];
+            auto load_k = [&](int c) {
+                page = c < c1 ? page_of(a.kv, b, c * TOK) : -1;
+                if (page < 0) return;
+                const int64_t tile = (int64_t)page * H + h;
+                const uint8_t* kp = static_cast<const uint8_t*>(a.kv.k) + tile * kKv8Page * D + (int64_t)(c % CPP) * kMassChunk;
+#pragma unroll
+                for (int n = 0; n < NB; ++n) {
+                    ks_next[n] = __ldg(a.kv.k_scale + tile * kKv8Blocks + (c % CPP) * NB + n);
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) k_codes<D>(kp + (n * 16 + slot_of(gq >> 1, gq & 1, j)) * D, w[n][j]);
+                }
+            };
+            load_k(c0 + warp);
             __syncthreads();  // the tiles before these are done with
             if (warp < nt) {
                 const int row0 = (tb + warp) * 16;
@@ -1052,27 +1121,17 @@ __global__ void __launch_bounds__(kThreads) kv8_mass_kernel(const __grid_constan
             }
             __syncthreads();
             for (int c = c0 + warp; c < c1; c += kWarps) {
-                const int page = page_of(a.kv, b, c * TOK);
                 float sum[NB][2][2] = {};
                 if (page >= 0 && nt > 0) {
-                    const int64_t tile = (int64_t)page * H + h;
-                    const uint8_t* kp = static_cast<const uint8_t*>(a.kv.k) + tile * kKv8Page * D + (int64_t)(c % CPP) * kMassChunk;
                     uint32_t kf[NB][2][KS][2];
                     float ks[NB];
-                    {
-                        uint32_t w[NB][2][KS];
 #pragma unroll
-                        for (int n = 0; n < NB; ++n) {
-                            ks[n] = __ldg(a.kv.k_scale + tile * kKv8Blocks + (c % CPP) * NB + n);
+                    for (int n = 0; n < NB; ++n) {
+                        ks[n] = ks_next[n];
 #pragma unroll
-                            for (int j = 0; j < 2; ++j) k_codes<D>(kp + (n * 16 + slot_of(gq >> 1, gq & 1, j)) * D, w[n][j]);
-                        }
+                        for (int j = 0; j < 2; ++j)
 #pragma unroll
-                        for (int n = 0; n < NB; ++n)
-#pragma unroll
-                            for (int j = 0; j < 2; ++j)
-#pragma unroll
-                                for (int k = 0; k < KS; ++k) widen<FMT>(w[n][j][k], kf[n][j][k][0], kf[n][j][k][1]);
+                            for (int k = 0; k < KS; ++k) widen<FMT>(w[n][j][k], kf[n][j][k][0], kf[n][j][k][1]);
                     }
                     for (int t = 0; t < nt; ++t) {
                         const bool whole = c * TOK + TOK <= rvis[t * 16];
@@ -1126,6 +1185,7 @@ __global__ void __launch_bounds__(kThreads) kv8_mass_kernel(const __grid_constan
                     if (t < s.len) a.mass_out[at] = (in ? in[at] : 0.0f) + sums[i];
                 }
                 __syncwarp();
+                load_k(c + kWarps);
             }
         }
         pos += c1 - c0;
@@ -1152,15 +1212,15 @@ struct AttendLaunch {
         a.shares = sm_count() * (RW == 1 ? 1 : SH::GROUPS);
         cudaError_t e = kv8_launch<kv8_attend_kernel<FMT, D, FEW, RW, F32>>(dim3(sm_count()), SH::THREADS, SH::SMEM, 1, s, a);
         if (e != cudaSuccess) return e;
+        if (a.scores) {
+            const dim3 blocks(min(64, (a.kv.max_pages * kKv8Page + 511) / 512), a.kv.kv_heads, a.kv.n_seqs);
+            return kv8_launch<kv8_weights_kernel<D, F32>>(blocks, 128, 0, 1, s, a);
+        }
         const int64_t rows = (int64_t)a.max_new * a.heads;
         const dim3 grid((unsigned)min((int64_t)1024, (rows + kWarps - 1) / kWarps), a.kv.n_seqs);
         e = kv8_launch<kv8_merge_kernel<D, FEW, RW, F32>>(grid, kThreads, 0, 1, s, a);
         if (e != cudaSuccess || !a.mass_out) return e;
-        if (a.scores) {
-            const dim3 blocks(min(64, (a.kv.max_pages * kKv8Page + 511) / 512), a.kv.kv_heads, a.kv.n_seqs);
-            return kv8_launch<kv8_weights_kernel<D>>(blocks, 128, 0, 1, s, a);
-        }
-        return kv8_launch<kv8_mass_kernel<FMT, D, F32>>(dim3(2 * sm_count()), kThreads, mass_smem<D, F32>(), 1, s, a);
+        return kv8_launch<kv8_mass_kernel<FMT, D, F32>>(dim3(sm_count()), kThreads, mass_smem<D, F32>(), 1, s, a);
     }
     template <int FMT, int D, bool FEW, int RW>
     cudaError_t by_type() {
@@ -1171,9 +1231,7 @@ struct AttendLaunch {
         switch (row_warps((int64_t)a.max_new * a.group)) {
         case 0: return by_type<FMT, D, true, 1>();
         case 1: return by_type<FMT, D, false, 1>();
-        case 2: return by_type<FMT, D, false, 2>();
-        case 4: return by_type<FMT, D, false, 4>();
-        default: return by_type<FMT, D, false, 8>();
+        default: return by_type<FMT, D, false, 2>();
         }
     }
 };
