@@ -1035,10 +1035,10 @@ __global__ void __launch_bounds__(128) kv8_weights_kernel(const __grid_constant_
 }
 
 // ---- accumulated weights, from K ------------------------------------------------------------------------------------------
-// More query rows: the scores are computed again, with the finished softmax sums at hand.  CTAs take equal consecutive
-// shares of the (sequence, KV head, chunk) list; a warp holds a chunk's K in registers as f16 and runs the query tiles
-// past it from shared memory.
-constexpr int kMassTiles = kWarps, kMassChunk = 4096;  // query tiles in shared memory, one loaded by each warp; K codes a warp holds
+// More query rows: the scores are computed again, with the finished softmax sums at hand.  The chunks of each sequence and
+// KV head are dealt to the warps of gridDim.x CTAs; a warp holds a chunk's K in registers as f16 and runs the query tiles
+// past it from shared memory.  Two CTAs an SM, with half the chunk that one would take: latency is what bounds it.
+constexpr int kMassTiles = kWarps, kMassChunk = 2048;  // query tiles in shared memory, one loaded by each warp; K codes a warp holds
 
 template <int D, bool F32>
 constexpr size_t mass_smem() {
@@ -1046,7 +1046,7 @@ constexpr size_t mass_smem() {
 }
 
 template <int FMT, int D, bool F32>
-__global__ void __launch_bounds__(kThreads) kv8_mass_kernel(const __grid_constant__ Kv8AttendArgs a) {
+__global__ void __launch_bounds__(kThreads, 2) kv8_mass_kernel(const __grid_constant__ Kv8AttendArgs a) {
     constexpr int TOK = kMassChunk / D, NB = TOK / kKv8Block, CPP = kKv8Page / TOK, KS = D / 16;
     extern __shared__ __align__(128) unsigned char smem[];
     pdl_wait();
@@ -1058,137 +1058,119 @@ __global__ void __launch_bounds__(kThreads) kv8_mass_kernel(const __grid_constan
     float* sums = reinterpret_cast<float*>(rvis + kMassTiles * 16) + (threadIdx.x >> 5) * 64;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gq = lane >> 2, c4 = lane & 3, H = a.kv.kv_heads;
     const bool vq = vec_rows(a.q);
-    const auto chunks_of = [&](int b) { return (seq_of<TOK, 16>(a, b).len + TOK - 1) / TOK; };
-    int total = 0, pos = 0, end = 0, b, base = 0;  // base: where sequence b's items start
-    find_part<kThreads>(
-        reinterpret_cast<int*>(smem), a.kv.n_seqs, [&](int i) { return H * chunks_of(i); },
-        [&](int sum) {
-            const int per = share_of(sum, gridDim.x);
-            pos = min(sum, (int)blockIdx.x * per), end = min(sum, pos + per);
-            return pos;
-        },
-        [](int, int) {}, total, b, base);
-    while (pos < end) {
-        const Seq s = seq_of<TOK, 16>(a, b);
-        const int chunks = (s.len + TOK - 1) / TOK;
-        if (pos >= base + H * chunks) {
-            base += H * chunks;
-            ++b;
-            continue;
+    const int b = blockIdx.z, h = blockIdx.y;
+    const Seq s = seq_of<TOK, 16>(a, b);
+    const int chunks = (s.len + TOK - 1) / TOK, c0 = blockIdx.x * kWarps, rows = s.n * a.group, tiles = s.tiles;
+    if (c0 >= chunks) return;
+    for (int tb = 0; tb < max(1, tiles); tb += kMassTiles) {
+        const int nt = min(kMassTiles, tiles - tb);
+        // a chunk's K codes as they are stored: the first is on its way while the rows are made ready
+        int page = -1;
+        uint32_t w[NB][2][KS];
+        float ks_next[NB];
+        auto load_k = [&](int c) {
+            page = c < chunks ? page_of(a.kv, b, c * TOK) : -1;
+            if (page < 0) return;
+            const int64_t tile = (int64_t)page * H + h;
+            const uint8_t* kp = static_cast<const uint8_t*>(a.kv.k) + tile * kKv8Page * D + (int64_t)(c % CPP) * kMassChunk;
+#pragma unroll
+            for (int n = 0; n < NB; ++n) {
+                ks_next[n] = __ldg(a.kv.k_scale + tile * kKv8Blocks + (c % CPP) * NB + n);
+#pragma unroll
+                for (int j = 0; j < 2; ++j) k_codes<D>(kp + (n * 16 + slot_of(gq >> 1, gq & 1, j)) * D, w[n][j]);
+            }
+        };
+        load_k(c0 + warp);
+        __syncthreads();  // the tiles before these are done with
+        if (warp < nt) {
+            const int row0 = (tb + warp) * 16;
+            QFrag<D, 2, F32> q;
+            QRaw<D, 2, F32> raw;
+            raw.fetch(a, s, h, row0, vq);
+            q.convert(raw, a.scale);
+#pragma unroll
+            for (int k = 0; k < KS; ++k) {
+                qs[(warp * KS + k) * 32 + lane] = make_uint4(q.hi[k][0], q.hi[k][1], q.hi[k][2], q.hi[k][3]);
+                const uint32_t(&lo)[4] = q.lo[F32 ? k : 0];
+                if (F32) qs[((kMassTiles + warp) * KS + k) * 32 + lane] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+            }
+            if (c4 == 0)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int r = row0 + gq + 8 * e, at = warp * 16 + gq + 8 * e, i = r / a.group;
+                    rfac[at] = q.factor[e];
+                    rvis[at] = visible(a, s, r);
+                    rlse[at] = r < rows ? __ldcg(a.lse + (int64_t)(s.first + i) * a.heads + h * a.group + r - i * a.group) : INFINITY;
+                }
         }
-        const int h = (pos - base) / chunks, c0 = (pos - base) % chunks, c1 = min(chunks, c0 + (end - pos));
-        const int rows = s.n * a.group, tiles = s.tiles;
-        for (int tb = 0; tb < max(1, tiles); tb += kMassTiles) {
-            const int nt = min(kMassTiles, tiles - tb);
-            // a chunk's K codes as they are stored: the first is on its way while the rows are made ready
-            int page = -1;
-            uint32_t w[NB][2][KS];
-            float ks_next[NB];
-            auto load_k = [&](int c) {
-                page = c < c1 ? page_of(a.kv, b, c * TOK) : -1;
-                if (page < 0) return;
-                const int64_t tile = (int64_t)page * H + h;
-                const uint8_t* kp = static_cast<const uint8_t*>(a.kv.k) + tile * kKv8Page * D + (int64_t)(c % CPP) * kMassChunk;
+        __syncthreads();
+        for (int c = c0 + warp; c < chunks; c += gridDim.x * kWarps) {
+            float sum[NB][2][2] = {};
+            if (page >= 0 && nt > 0) {
+                uint32_t kf[NB][2][KS][2];
+                float ks[NB];
 #pragma unroll
                 for (int n = 0; n < NB; ++n) {
-                    ks_next[n] = __ldg(a.kv.k_scale + tile * kKv8Blocks + (c % CPP) * NB + n);
+                    ks[n] = ks_next[n];
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) k_codes<D>(kp + (n * 16 + slot_of(gq >> 1, gq & 1, j)) * D, w[n][j]);
+                    for (int j = 0; j < 2; ++j)
+#pragma unroll
+                        for (int k = 0; k < KS; ++k) widen<FMT>(w[n][j][k], kf[n][j][k][0], kf[n][j][k][1]);
                 }
-            };
-            load_k(c0 + warp);
-            __syncthreads();  // the tiles before these are done with
-            if (warp < nt) {
-                const int row0 = (tb + warp) * 16;
-                QFrag<D, 2, F32> q;
-                QRaw<D, 2, F32> raw;
-                raw.fetch(a, s, h, row0, vq);
-                q.convert(raw, a.scale);
+                for (int t = 0; t < nt; ++t) {
+                    const bool whole = c * TOK + TOK <= rvis[t * 16];
+                    uint4 q[KS], p[F32 ? KS : 1];
 #pragma unroll
-                for (int k = 0; k < KS; ++k) {
-                    qs[(warp * KS + k) * 32 + lane] = make_uint4(q.hi[k][0], q.hi[k][1], q.hi[k][2], q.hi[k][3]);
-                    const uint32_t(&lo)[4] = q.lo[F32 ? k : 0];
-                    if (F32) qs[((kMassTiles + warp) * KS + k) * 32 + lane] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-                }
-                if (c4 == 0)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const int r = row0 + gq + 8 * e, at = warp * 16 + gq + 8 * e, i = r / a.group;
-                        rfac[at] = q.factor[e];
-                        rvis[at] = visible(a, s, r);
-                        rlse[at] = r < rows ? __ldcg(a.lse + (int64_t)(s.first + i) * a.heads + h * a.group + r - i * a.group) : INFINITY;
+                    for (int k = 0; k < KS; ++k) {
+                        q[k] = qs[(t * KS + k) * 32 + lane];
+                        if (F32) p[F32 ? k : 0] = qs[((kMassTiles + t) * KS + k) * 32 + lane];
                     }
-            }
-            __syncthreads();
-            for (int c = c0 + warp; c < c1; c += kWarps) {
-                float sum[NB][2][2] = {};
-                if (page >= 0 && nt > 0) {
-                    uint32_t kf[NB][2][KS][2];
-                    float ks[NB];
+                    const float fac[2] = {rfac[t * 16 + gq], rfac[t * 16 + gq + 8]};
+                    const float lse[2] = {rlse[t * 16 + gq], rlse[t * 16 + gq + 8]};
+                    const int vis[2] = {rvis[t * 16 + gq], rvis[t * 16 + gq + 8]};
 #pragma unroll
-                    for (int n = 0; n < NB; ++n) {
-                        ks[n] = ks_next[n];
+                    for (int n = 0; n < NB; ++n)
 #pragma unroll
-                        for (int j = 0; j < 2; ++j)
+                        for (int j = 0; j < 2; ++j) {
+                            float x[4];
+                            score_sum<KS, F32>(x, [&](float (&y)[4], int k, bool second) {
+                                const uint4& r = second ? p[F32 ? k : 0] : q[k];
+                                mma_f16(y, r.x, r.y, r.z, r.w, kf[n][j][k][0], kf[n][j][k][1]);
+                            });
 #pragma unroll
-                            for (int k = 0; k < KS; ++k) widen<FMT>(w[n][j][k], kf[n][j][k][0], kf[n][j][k][1]);
-                    }
-                    for (int t = 0; t < nt; ++t) {
-                        const bool whole = c * TOK + TOK <= rvis[t * 16];
-                        uint4 q[KS], p[F32 ? KS : 1];
-#pragma unroll
-                        for (int k = 0; k < KS; ++k) {
-                            q[k] = qs[(t * KS + k) * 32 + lane];
-                            if (F32) p[F32 ? k : 0] = qs[((kMassTiles + t) * KS + k) * 32 + lane];
-                        }
-                        const float fac[2] = {rfac[t * 16 + gq], rfac[t * 16 + gq + 8]};
-                        const float lse[2] = {rlse[t * 16 + gq], rlse[t * 16 + gq + 8]};
-                        const int vis[2] = {rvis[t * 16 + gq], rvis[t * 16 + gq + 8]};
-#pragma unroll
-                        for (int n = 0; n < NB; ++n)
-#pragma unroll
-                            for (int j = 0; j < 2; ++j) {
-                                float x[4];
-                                score_sum<KS, F32>(x, [&](float (&y)[4], int k, bool second) {
-                                    const uint4& r = second ? p[F32 ? k : 0] : q[k];
-                                    mma_f16(y, r.x, r.y, r.z, r.w, kf[n][j][k][0], kf[n][j][k][1]);
-                                });
-#pragma unroll
-                                for (int i = 0; i < 4; ++i) {
-                                    float v = ex2(x[i] * (fac[i >> 1] * ks[n]) - lse[i >> 1]);
-                                    if (!whole && c * TOK + n * 16 + slot_of(c4, i & 1, j) >= vis[i >> 1]) v = 0.0f;
-                                    sum[n][j][i & 1] += v;
-                                }
+                            for (int i = 0; i < 4; ++i) {
+                                float v = ex2(x[i] * (fac[i >> 1] * ks[n]) - lse[i >> 1]);
+                                if (!whole && c * TOK + n * 16 + slot_of(c4, i & 1, j) >= vis[i >> 1]) v = 0.0f;
+                                sum[n][j][i & 1] += v;
                             }
-                    }
-#pragma unroll
-                    for (int n = 0; n < NB; ++n)
-#pragma unroll
-                        for (int j = 0; j < 2; ++j)
-#pragma unroll
-                            for (int e = 0; e < 2; ++e)
-#pragma unroll
-                                for (int x = 4; x < 32; x <<= 1) sum[n][j][e] += __shfl_xor_sync(0xffffffffu, sum[n][j][e], x);
+                        }
                 }
-                if (gq == 0)
 #pragma unroll
-                    for (int n = 0; n < NB; ++n)
+                for (int n = 0; n < NB; ++n)
 #pragma unroll
-                        for (int j = 0; j < 2; ++j)
+                    for (int j = 0; j < 2; ++j)
 #pragma unroll
-                            for (int e = 0; e < 2; ++e) sums[n * 16 + slot_of(c4, e, j)] = sum[n][j][e];
-                __syncwarp();
-                const float* in = tb ? a.mass_out : a.mass_in;
-                for (int i = lane; i < TOK; i += 32) {
-                    const int t = c * TOK + i;
-                    const int64_t at = ((int64_t)b * H + h) * a.mass_stride + t;
-                    if (t < s.len) a.mass_out[at] = (in ? in[at] : 0.0f) + sums[i];
-                }
-                __syncwarp();
-                load_k(c + kWarps);
+                        for (int e = 0; e < 2; ++e)
+#pragma unroll
+                            for (int x = 4; x < 32; x <<= 1) sum[n][j][e] += __shfl_xor_sync(0xffffffffu, sum[n][j][e], x);
             }
+            if (gq == 0)
+#pragma unroll
+                for (int n = 0; n < NB; ++n)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) sums[n * 16 + slot_of(c4, e, j)] = sum[n][j][e];
+            __syncwarp();
+            const float* in = tb ? a.mass_out : a.mass_in;
+            for (int i = lane; i < TOK; i += 32) {
+                const int t = c * TOK + i;
+                const int64_t at = ((int64_t)b * H + h) * a.mass_stride + t;
+                if (t < s.len) a.mass_out[at] = (in ? in[at] : 0.0f) + sums[i];
+            }
+            __syncwarp();
+            load_k(c + gridDim.x * kWarps);
         }
-        pos += c1 - c0;
     }
 }
 
@@ -1220,7 +1202,9 @@ struct AttendLaunch {
         const dim3 grid((unsigned)min((int64_t)1024, (rows + kWarps - 1) / kWarps), a.kv.n_seqs);
         e = kv8_launch<kv8_merge_kernel<D, FEW, RW, F32>>(grid, kThreads, 0, 1, s, a);
         if (e != cudaSuccess || !a.mass_out) return e;
-        return kv8_launch<kv8_mass_kernel<FMT, D, F32>>(dim3(sm_count()), kThreads, mass_smem<D, F32>(), 1, s, a);
+        const int units = a.kv.kv_heads * a.kv.n_seqs, most = (a.kv.max_pages * (kKv8Page * D / kMassChunk) + kWarps - 1) / kWarps;
+        const dim3 parts(max(1, min((2 * sm_count() + units - 1) / units, most)), a.kv.kv_heads, a.kv.n_seqs);
+        return kv8_launch<kv8_mass_kernel<FMT, D, F32>>(parts, kThreads, mass_smem<D, F32>(), 1, s, a);
     }
     template <int FMT, int D, bool FEW, int RW>
     cudaError_t by_type() {
