@@ -115,6 +115,9 @@ struct Shape {
     static constexpr int NB = TOK / kKv8Block, CPP = kKv8Page / TOK; // blocks of a chunk, chunks of a page
     static constexpr int STAGES = FEW ? 3 : RW == 1 ? 2 : 6;
     static constexpr int PART = D + 4;  // floats of one row's partial result: its sums, then M, R and l
+    // items of a share: a chunk for each warp, and of groups enough that merging does not cost more than they do (one
+    // sequence of 2048 slots: 32 CTAs and 4 parts a unit, not 128 and 16)
+    static constexpr int LEAST = RW == 1 ? WARPS : 4;
     static constexpr int BARS = RW == 1 ? 1 : 2;  // a warp on its own needs no barrier to hand stages back
     static constexpr size_t HEAD = RW == 1 ? (size_t)ROWS * PART * sizeof(float) : 0;
     static constexpr size_t SMEM = (size_t)GROUPS * (STAGES * (2 * CHUNK + 8 * sizeof(float) + BARS * 8 + 4) + HEAD);
@@ -143,8 +146,8 @@ LDEV Seq seq_of(const Kv8AttendArgs& a, int b) {
     return s;
 }
 
-// items of one share when `total` are dealt to n shares
-LDEV int share_of(int total, int n) { return (int)(((unsigned)total + n - 1) / n); }
+// items of one share when `total` are dealt to n shares, `least` or more to each
+LDEV int share_of(int total, int n, int least) { return max(least, (int)(((unsigned)total + n - 1) / n)); }
 
 // exclusive prefix sum of v over the block and the total; `red` holds 32 ints
 template <int THREADS>
@@ -651,15 +654,26 @@ LDEV void add_parts(int n, At at, float (&o)[D / 32], float& M, float& R, float&
     const float old = pow2i(R - Rn), mine = pow2i(m.y - Rn);
 #pragma unroll
     for (int e = 0; e < V; ++e) o[e] *= old;
-#pragma unroll 8
-    for (int i = 0; i < n; ++i) {
-        const float f = __shfl_sync(0xffffffffu, mine, i);
-        if (V == 2) {
-            const float2 x = reinterpret_cast<const float2*>(at(i))[lane];
-            o[0] += x.x * f, o[1] += x.y * f;
-        } else {
-            const float4 x = reinterpret_cast<const float4*>(at(i))[lane];
-            o[0] += x.x * f, o[1] += x.y * f, o[V - 2] += x.z * f, o[V - 1] += x.w * f;
+    for (int i0 = 0; i0 < n; i0 += 8) {  // eight parts' loads on their way at a time
+        float x[8][V];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+#pragma unroll
+            for (int e = 0; e < V; ++e) x[i][e] = 0.0f;
+            if (i0 + i < n) {
+                const float* p = at(i0 + i) + lane * V;
+                if (V == 2)
+                    *reinterpret_cast<float2*>(x[i]) = *reinterpret_cast<const float2*>(p);
+                else
+                    *reinterpret_cast<float4*>(x[i]) = *reinterpret_cast<const float4*>(p);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float f = __shfl_sync(0xffffffffu, mine, i0 + i);
+#pragma unroll
+            for (int e = 0; e < V; ++e)
+                if (i0 + i < n) o[e] += x[i][e] * f;
         }
     }
     M = Mn;
@@ -731,11 +745,11 @@ __global__ void __launch_bounds__(Shape<D, FEW, RW>::THREADS, 1) kv8_attend_kern
         },
         [&](int sum) {
             if (RW == 1) {
-                const int per = share_of(sum, gridDim.x), lo = min(sum, (int)blockIdx.x * per), hi = min(sum, lo + per);
-                const int each = share_of(hi - lo, SH::WARPS);
+                const int per = share_of(sum, gridDim.x, SH::LEAST), lo = min(sum, (int)blockIdx.x * per), hi = min(sum, lo + per);
+                const int each = share_of(hi - lo, SH::WARPS, 1);
                 beg = min(hi, lo + warp * each), end = min(hi, beg + each);
             } else {  // groups of one CTA are far apart in the list, so that a short one still uses every SM
-                const int per = share_of(sum, gridDim.x * SH::GROUPS);
+                const int per = share_of(sum, gridDim.x * SH::GROUPS, SH::LEAST);
                 beg = min(sum, (wg * (int)gridDim.x + (int)blockIdx.x) * per), end = min(sum, beg + per);
             }
             return beg;
@@ -953,7 +967,7 @@ __global__ void __launch_bounds__(kThreads) kv8_merge_kernel(const __grid_consta
     pdl_launch();
     const int b = blockIdx.y;
     const Seq s = seq_of<SH::TOK, SH::TILE>(a, b);
-    const int per = share_of(a.offset[a.kv.n_seqs], a.shares), base = a.offset[b];
+    const int per = share_of(a.offset[a.kv.n_seqs], a.shares, SH::LEAST), base = a.offset[b];
     for (int u = blockIdx.x * kWarps + (threadIdx.x >> 5); u < s.n * a.heads; u += gridDim.x * kWarps) {
         const int i = u / a.heads, hq = u - i * a.heads, h = hq / a.group, r = i * a.group + hq - h * a.group, tile = r / SH::TILE;
         const int first = base + (h * s.tiles + tile) * s.chunks, g0 = first / per, g1 = (first + s.chunks - 1) / per;
@@ -980,7 +994,7 @@ __global__ void __launch_bounds__(128) kv8_weights_kernel(const __grid_constant_
     const int b = blockIdx.z, h = blockIdx.y, H = a.kv.kv_heads, lane = threadIdx.x & 31;
     const Seq s = seq_of<SH::TOK, SH::TILE>(a, b);
     const int base = a.offset[b] + h * s.chunks, rows = s.n * a.group;
-    const int per = share_of(a.offset[a.kv.n_seqs], a.shares), g0 = rows ? base / per : 0, g1 = rows ? (base + s.chunks - 1) / per : 0;
+    const int per = share_of(a.offset[a.kv.n_seqs], a.shares, SH::LEAST), g0 = rows ? base / per : 0, g1 = rows ? (base + s.chunks - 1) / per : 0;
     if (blockIdx.x * 512 >= s.len && blockIdx.x > 0) return;
     for (int r = threadIdx.x >> 5; r < rows; r += 4) {
         if (g0 == g1) {
