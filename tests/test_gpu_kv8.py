@@ -366,6 +366,81 @@ def test_pools_beyond_two_gigabytes(ctx):
     check_attend(gpu, ref, rng, [150], [1], 16, "bf16")
 
 
+def test_more_sequences_than_a_block_has_threads(ctx):
+    """the list of work is found in several steps; sequences without queries or slots among them"""
+    rng = np.random.default_rng(12)
+    lens = rng.integers(0, 40, 700).tolist()
+    lens[255], lens[256], lens[511], lens[512] = 64, 1, 0, 130
+    news = [min(n, int(m)) for n, m in zip(lens, rng.integers(0, 3, 700))]
+    gpu, ref, rng = filled(ctx, "int8", 1, 64, lens)
+    check_attend(gpu, ref, rng, lens, news, 2, "f32")  # few rows
+    check_attend(gpu, ref, rng, lens, [4 * n for n in news], 5, "bf16")  # many rows, also more queries than slots
+
+
+@pytest.mark.parametrize("kv,group,d,dtype,new", [(1, 4, 128, "bf16", 1), (1, 2, 64, "f32", 3), (1, 9, 64, "bf16", 1), (1, 12, 128, "bf16", 3)])
+def test_one_long_sequence_in_many_parts(ctx, kv, group, d, dtype, new):
+    """more parts of one unit than a warp has lanes"""
+    lens = [40001]
+    gpu, ref, rng = filled(ctx, "e4m3", kv, d, lens)
+    check_attend(gpu, ref, rng, lens, [new], kv * group, dtype)
+    check_attend(gpu, ref, rng, lens, [new], kv * group, dtype, with_mass=False)
+
+
+def test_weights_rebuilt_from_k_when_scores_are_not_kept(ctx):
+    """a page table so long that the scores of every slot it could name would pass the workspace's bound"""
+    kv, d, heads, pages = 8, 64, 64, 70000
+    gpu, ref, rng = filled(ctx, "e4m3", kv, d, [300])
+    scores = lambda: gpu.c.attend_workspace(heads, 1, True) - gpu.c.attend_workspace(heads, 1, False)  # noqa: E731
+    assert scores() > kv * 300 * heads // kv * 4
+    wide = torch.full((1, pages), 2 ** 30, dtype=torch.int32, device="cuda")
+    wide[:, :gpu.table.shape[1]] = gpu.table
+    gpu.c = LB.Kv8Cache(ctx, "e4m3", 1, kv, d, gpu.num_pages, pages, gpu.k, gpu.v, gpu.ks, gpu.vs, wide, gpu.status)
+    assert scores() < 2 ** 12
+    check_attend(gpu, ref, rng, [300], [1], heads, "f32")
+    check_attend(gpu, ref, rng, [300], [1], heads, "bf16", stride=301)
+
+
+@pytest.mark.parametrize("group,new", [(3, 1), (5, 4)])
+def test_scales_of_either_sign_and_zero(ctx, group, new):
+    lens = [100, 33]
+    gpu, ref, rng = filled(ctx, "int8", 1, 64, lens)
+    q = [rows(rng, new, group, 64, "f32") for _ in lens]
+    for scale in (-0.125, 0.0, -0.0, 1e-30):
+        out, mass = gpu.attend(lens, q, scale, mass=True, stride=101)
+        for b, n in enumerate(lens):
+            want, wm, big = ref.attend(b, f64(q[b]), scale)
+            vmax = max(np.abs(ref.side[b][0]["v"].values()).max(), 0.0)
+            rel, tol = bounds("f32", 64, big, vmax)
+            assert (np.abs(f64(out[b * new:(b + 1) * new]) - want) <= tol).all()
+            assert (np.abs(f64(mass[b, :, :n]) - wm) <= rel * wm + 2.0 ** -22 * wm).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("group,new", [(2, 1), (6, 3)])
+def test_values_of_very_different_size(ctx, dtype, group, new):
+    """V blocks from 1e-30 to 1e30, the large ones far out of the attention, zeros where it looks: weights stay in range"""
+    n, d = 128, 64
+    rng = np.random.default_rng(8)
+    k = np.zeros((n, 1, d))
+    v = rng.standard_normal((n, 1, d))
+    k[:, 0, 0] = np.repeat([0.0, -300.0, 1.0, -300.0, 2.0, 0.5, -300.0, 3.0], 16)
+    v *= np.repeat([1.0, 1e30, 1e-4, 1e38, 1e-30, 2.0, 1e20, 0.0], 16)[:, None, None]
+    k, v = (torch.tensor(x, dtype=torch.float32) for x in (k, v))
+    gpu, ref = Gpu(ctx, "e4m3", 1, 1, d, 2), R.Cache(1, 1, d, "e4m3")
+    gpu.append([0], [k.cuda()], [v.cuda()])
+    ref.append(0, f64(k), f64(v))
+    q = torch.zeros(new, group, d)
+    q[:, :, 0] = 1.0
+    q[:, :, 1:] = torch.tensor(rng.standard_normal((new, group, d - 1)))
+    q = q.to(DT[dtype]).cuda()
+    out, mass = gpu.attend([n], [q], 1.0, mass=True)
+    want, wm, big = ref.attend(0, f64(q), 1.0)
+    # what each query sees: the far blocks' weights are e^-300 = 0 against values of at most 1e38; the blocks near 1 rule
+    rel, tol = bounds(dtype, d, big, 10.0)
+    assert (np.abs(f64(out) - want) <= tol + 2.0 ** -8 * np.abs(want)).all()
+    assert (np.abs(f64(mass[0]) - wm) <= rel * wm + 1e-12).all()
+
+
 # ---- eviction ---------------------------------------------------------------------------------------------------------
 def check_evict(ctx, gpu, ref, lens, mass, budget, recent, stride_out=None):
     n, kv, d = len(lens), gpu.kv, gpu.d
@@ -438,6 +513,27 @@ def test_eviction_from_long_contexts(ctx, length, budget, recent):
         want = torch.cat([order.cpu(), torch.arange(cand, length)])
         assert torch.equal(kept[0, h].cpu().long(), want)
         assert np.array_equal(got[0, :, h], k[0, want.numpy(), h])
+
+
+@pytest.mark.parametrize("length,shift", [(150001, 0), (200000, 1), (30000, 1), (3000, 3)])
+def test_eviction_with_masses_at_any_address(ctx, length, shift):
+    """mass rows off 16-byte boundaries, and more slots than a cluster's shared memory holds the keys of"""
+    rng = np.random.default_rng(length)
+    flat = torch.tensor(rng.standard_normal(length + shift), dtype=torch.float32).cuda()
+    mass = flat[shift:].view(1, 1, length)
+    gpu = Gpu(ctx, "e4m3", 1, 1, 64, -(-length // R.PAGE))
+    gpu.k.random_(0, 127), gpu.v.random_(0, 127), gpu.ks.fill_(1.0), gpu.vs.fill_(0.25)
+    budget, recent = length // 3, 77
+    dst = Gpu(ctx, "e4m3", 1, 1, 64, -(-budget // R.PAGE), seed=3)
+    kept, out = torch.zeros(1, 1, budget, dtype=torch.int32, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
+    mo = torch.zeros(1, 1, budget, device="cuda")
+    gpu.c.evict(dst.c, ints([length]), budget, recent, mass, length, kept, out, mo, budget)
+    order = torch.sort(mass[0, 0, :length - recent], descending=True, stable=True).indices[:budget - recent].sort().values
+    want = torch.cat([order, torch.arange(length - recent, length, device="cuda")])
+    assert torch.equal(kept[0, 0].long(), want) and torch.equal(mo[0, 0], mass[0, 0, want])
+    k, _ = gpu.values([length])
+    got, _ = dst.values([budget])
+    assert np.array_equal(got[0, :, 0], k[0, want.cpu().numpy(), 0])
 
 
 def test_a_bounded_cache_decodes_on(ctx):
