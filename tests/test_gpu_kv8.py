@@ -565,6 +565,25 @@ def test_a_bounded_cache_decodes_on(ctx):
                 mass = torch.zeros(3, kv, 128, device="cuda")
 
 
+def test_the_bounded_decode_example(ctx):
+    """without evictions a bounded cache decodes like a large one; with them it runs on in the same memory"""
+    import importlib.util
+    import os
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "bounded_decode.py")
+    spec = importlib.util.spec_from_file_location("bounded_decode", path)
+    ex = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(ex)
+    for fmt in R.QMAX:
+        large, c = ex.decode(3, 150, 256, 64, 16, fmt)
+        assert c.evictions == 0
+        small, c = ex.decode(3, 150, 96, 64, 16, fmt)
+        assert c.evictions == 2 and c.longest == 64 + (150 - 96 - 32) and c.slots == 128
+        assert torch.equal(small[:, :96], large[:, :96])
+        # after 150 steps of 16 heads the kept slots hold at most the weight handed out since the start
+        total = c.mass[0][:, :, :c.longest].double().sum(-1)
+        assert (total <= 150 * 2 + 1e-3).all() and (total > 0).all()
+
+
 # ---- streams, refusals, bad data on the device ------------------------------------------------------------------------
 def test_a_context_on_its_own_stream(ctx):
     side = torch.cuda.Stream()
