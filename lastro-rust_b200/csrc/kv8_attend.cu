@@ -449,7 +449,8 @@ struct WarpRows {
                 float top = s[b][e][0];
 #pragma unroll
                 for (int k = 1; k < NT; ++k) top = fmaxf(top, s[b][e][k]);
-                top *= fk[b][e];
+                // a block that was never written has any scale, a negative one among them
+                top = !WHOLE && top == -INFINITY ? top : top * fk[b][e];
                 m = fmaxf(m, top);
                 r = fmaxf(r, top + (float)((int)(__float_as_uint(vs[b]) >> 23) - 127));
             }

@@ -323,6 +323,27 @@ def test_a_nan_block_reaches_only_the_queries_that_see_it(ctx):
             assert torch.equal(part[:4], clean.attend([52], [q], 0.125)[0][:4]) and part[4:].isnan().all()
 
 
+@pytest.mark.parametrize("scale", [-1.0, -math.inf, math.inf, 0.0, -3e38, 1e-40, math.nan])
+@pytest.mark.parametrize("group,new", [(2, 1), (5, 3)])
+def test_what_was_never_written_does_not_matter(ctx, scale, group, new):
+    """any scale and any code in blocks and slots past a sequence's length"""
+    lens = [3, 17, 40, 64, 81]
+    for code in (0x7f, 0xff, 0x80, 0x00):
+        for fmt in R.QMAX:
+            gpu, rng = Gpu(ctx, fmt, 5, 1, 64, 2), np.random.default_rng(6)
+            for t in (gpu.ks, gpu.vs):
+                t.fill_(scale)
+            for t in (gpu.k, gpu.v):
+                t.fill_(code)
+            ref = R.Cache(5, 1, 64, fmt)
+            k, v = ([rows(rng, n, 1, 64, "f32") for n in lens] for _ in "kv")
+            gpu.append([0] * 5, k, v)
+            for b in range(5):
+                ref.append(b, f64(k[b]), f64(v[b]))
+            check_attend(gpu, ref, rng, lens, [new] * 5, group, "f32")
+            same_values(gpu, ref, lens)
+
+
 def test_mass_accumulates_in_place_and_over_steps(ctx):
     lens = [65, 20]
     gpu, ref, rng = filled(ctx, "int8", 2, 64, lens)
