@@ -233,20 +233,28 @@ __global__ void __launch_bounds__(CL > 1 ? 1024 : 512) kv8_select_kernel(const _
     if (want == 0) return;  // the same for the whole cluster
 
     const int run = ((cand + CL - 1) / CL + 3) & ~3, lo = min(cand, rank * run), n = min(cand, lo + run) - lo;
-    const bool held = run <= kSelSlots;
-    if (held && (reinterpret_cast<uintptr_t>(mass) & 15) == 0) {
-#pragma unroll 4
-        for (int i = tid; i < n / 4; i += kSelThreads) {
-            const float4 m = __ldg(reinterpret_cast<const float4*>(mass + lo) + i);
-            reinterpret_cast<uint4*>(keys)[i] = make_uint4(mass_key(m.x), mass_key(m.y), mass_key(m.z), mass_key(m.w));
+    // the keys, four at a time; 0, which is no mass's key and below them all, past the last
+    const bool held = run <= kSelSlots, vec = (reinterpret_cast<uintptr_t>(mass) & 15) == 0;
+    const int n4 = (n + 3) / 4;
+    auto fetch = [&](int i) {
+        const float* p = mass + lo + 4 * i;
+        if (vec && 4 * i + 4 <= n) {
+            const float4 m = __ldg(reinterpret_cast<const float4*>(p));
+            return make_uint4(mass_key(m.x), mass_key(m.y), mass_key(m.z), mass_key(m.w));
         }
-        if (tid < (n & 3)) keys[n - 1 - tid] = mass_key(__ldg(mass + lo + n - 1 - tid));
-        __syncthreads();
-    } else if (held) {
-#pragma unroll 8
-        for (int i = tid; i < n; i += kSelThreads) keys[i] = mass_key(__ldg(mass + lo + i));
+        uint32_t k[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) k[q] = 4 * i + q < n ? mass_key(__ldg(p + q)) : 0u;
+        return make_uint4(k[0], k[1], k[2], k[3]);
+    };
+    if (held) {
+#pragma unroll 4
+        for (int i = tid; i < n4; i += kSelThreads) reinterpret_cast<uint4*>(keys)[i] = fetch(i);
     }
-    auto key = [&](int i) { return held ? keys[i] : mass_key(__ldg(mass + lo + i)); };
+    auto four = [&](int i, uint32_t (&k)[4]) {
+        const uint4 v = held ? reinterpret_cast<const uint4*>(keys)[i] : fetch(i);
+        k[0] = v.x, k[1] = v.y, k[2] = v.z, k[3] = v.w;
+    };
     if (CL > 1) {
         for (int i = tid; i < kSelBins; i += kSelThreads) both[i] = 0;
         cluster_sync();
@@ -259,10 +267,13 @@ __global__ void __launch_bounds__(CL > 1 ? 1024 : 512) kv8_select_kernel(const _
         for (int i = tid; i < bins; i += kSelThreads) hist[i] = 0;
         __syncthreads();
         const uint32_t mask = pass == 0 ? 0u : pass == 1 ? 0xfff00000u : 0xfffffc00u;
-#pragma unroll 8
-        for (int i = tid; i < n; i += kSelThreads) {
-            const uint32_t k = key(i);
-            if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & (bins - 1)], 1u);
+#pragma unroll 2
+        for (int i = tid; i < n4; i += kSelThreads) {
+            uint32_t k[4];
+            four(i, k);
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                if ((k[q] & mask) == prefix) atomicAdd(&hist[(k[q] >> shift) & (bins - 1)], 1u);
         }
         __syncthreads();
         if (CL > 1) {
@@ -310,12 +321,13 @@ __global__ void __launch_bounds__(CL > 1 ? 1024 : 512) kv8_select_kernel(const _
         need = found[1];
     }
     // kept: every key above prefix, and the first `need` at it
-    const int span = ((n + kSelWarps - 1) / kSelWarps + 31) & ~31, wlo = min(n, warp * span), whi = min(n, wlo + span);
+    const int span = (n4 + kSelWarps - 1) / kSelWarps, wlo = min(n4, warp * span), whi = min(n4, wlo + span);
     uint32_t up = 0, at = 0;
     for (int i = wlo + lane; i < whi; i += 32) {
-        const uint32_t k = key(i);
-        up += k > prefix;
-        at += k == prefix;
+        uint32_t k[4];
+        four(i, k);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) up += k[q] > prefix, at += k[q] == prefix;
     }
     up = __reduce_add_sync(0xffffffffu, up);
     at = __reduce_add_sync(0xffffffffu, at);
@@ -334,17 +346,30 @@ __global__ void __launch_bounds__(CL > 1 ? 1024 : 512) kv8_select_kernel(const _
     }
     for (int i0 = wlo; i0 < whi; i0 += 32) {
         const int i = i0 + lane;
-        const uint32_t k = i < whi ? key(i) : 0u;
-        const unsigned gt = __ballot_sync(0xffffffffu, i < whi && k > prefix), eq = __ballot_sync(0xffffffffu, i < whi && k == prefix);
-        const unsigned below = (1u << lane) - 1;
-        const uint32_t u = up + __popc(gt & below), t = at + __popc(eq & below);
-        if ((gt >> lane & 1) || ((eq >> lane & 1) && t < need)) {
-            const uint32_t pos = u + min(t, need);
-            kept[pos] = lo + i;
-            if (mout) mout[pos] = key_mass(k);
+        uint32_t k[4] = {}, mine = 0;  // keys above prefix in the low half, at it in the high half
+        if (i < whi) four(i, k);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) mine += (k[q] > prefix) + (k[q] == prefix ? 0x10000u : 0u);
+        uint32_t incl = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t t = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += t;
         }
-        up += __popc(gt);
-        at += __popc(eq);
+        uint32_t u = up + ((incl - mine) & 0xffffu), t = at + ((incl - mine) >> 16);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            if (k[q] > prefix || (k[q] == prefix && t < need)) {
+                const uint32_t pos = u + min(t, need);
+                kept[pos] = lo + 4 * i + q;
+                if (mout) mout[pos] = key_mass(k[q]);
+            }
+            u += k[q] > prefix;
+            t += k[q] == prefix;
+        }
+        const uint32_t all32 = __shfl_sync(0xffffffffu, incl, 31);
+        up += all32 & 0xffffu;
+        at += all32 >> 16;
     }
     if (CL > 1) cluster_sync();  // no CTA leaves while another reads its counts
 }
@@ -506,7 +531,7 @@ struct EvictLaunch {
         // a cluster where one CTA's shared memory might not hold the keys
         const int64_t slots = (int64_t)a.src.max_pages * kKv8Page;
         const int cl = slots > kSelSlots ? 8 : 1;
-        const size_t smem = ((size_t)min((slots + cl - 1) / cl + 3, (int64_t)kSelSlots) + (cl > 1 ? 3 : 1) * kSelBins) * sizeof(uint32_t);
+        const size_t smem = ((size_t)min(((slots + cl - 1) / cl + 3) & ~(int64_t)3, (int64_t)kSelSlots) + (cl > 1 ? 3 : 1) * kSelBins) * sizeof(uint32_t);
         const dim3 grid(cl, a.src.kv_heads, a.src.n_seqs);
         const cudaError_t e = cl > 1 ? kv8_launch<kv8_select_kernel<8>>(grid, 1024, smem, 8, s, a)
                                      : kv8_launch<kv8_select_kernel<1>>(grid, 512, smem, 1, s, a);
