@@ -805,7 +805,7 @@ _row_dtypes = {}  # the same by the dtype objects met so far
 
 def _dev(x):
     """A device address: an int, None, or anything with data_ptr() (a torch tensor)."""
-    return x if x is None or isinstance(x, int) else x.data_ptr()
+    return x if x is None or x.__class__ is int else x.data_ptr()
 
 
 def rows_of(t) -> Rows:
@@ -836,13 +836,19 @@ class Kv8Cache:
         self.buffers = (k, v, k_scale, v_scale, page_table, status)  # tensors live as long as the cache
         self.desc = Kv8Desc(KV8_FORMATS[fmt], n_seqs, kv_heads, head_dim, num_pages, max_pages,
                             *(_dev(x) for x in self.buffers))
+        # what a call of a few microseconds should not look up again
+        L = lib()
         self._kv = C.byref(self.desc)
+        self._append, self._attend, self._evict, self._read = (L.lastro_kv8_append, L.lastro_kv8_attend, L.lastro_kv8_evict,
+                                                               L.lastro_kv8_read)
 
     def append(self, lens, new_off, max_new: int, k: Rows, v: Rows, lens_out, mass=None, mass_stride: int = 0):
         """Quantise rows [new_off[b], new_off[b + 1]) of k and v into slots lens[b].. of each sequence
         (lastro_kv8_append)."""
-        self.ctx.check(lib().lastro_kv8_append(self.ctx.h, self._kv, _dev(lens), _dev(new_off), max_new, k, v,
-                                               _dev(lens_out), _dev(mass), mass_stride))
+        rc = self._append(self.ctx.h, self._kv, _dev(lens), _dev(new_off), max_new, k, v, _dev(lens_out), _dev(mass),
+                          mass_stride)
+        if rc:
+            self.ctx.check(rc)
 
     def attend_workspace(self, heads: int, max_new: int, with_mass: bool) -> int:
         """Bytes of workspace attend() needs."""
@@ -855,20 +861,24 @@ class Kv8Cache:
                workspace_bytes: int, mass_in=None, mass_out=None, mass_stride: int = 0):
         """out = softmax(scale * q k) v over the slots each query sees; mass_out = mass_in + the weights each slot
         received (lastro_kv8_attend)."""
-        self.ctx.check(lib().lastro_kv8_attend(self.ctx.h, self._kv, _dev(lens), _dev(q_off), max_new, heads, q, scale,
-                                               out, _dev(mass_in), _dev(mass_out), mass_stride, _dev(workspace),
-                                               workspace_bytes))
+        rc = self._attend(self.ctx.h, self._kv, _dev(lens), _dev(q_off), max_new, heads, q, scale, out, _dev(mass_in),
+                          _dev(mass_out), mass_stride, _dev(workspace), workspace_bytes)
+        if rc:
+            self.ctx.check(rc)
 
     def evict(self, dst: "Kv8Cache", lens, budget: int, recent: int, mass, mass_stride: int, kept, lens_out,
               mass_out=None, mass_out_stride: int = 0):
         """Cut every sequence to `budget` slots by accumulated mass, its kept rows written to dst's pages
         (lastro_kv8_evict)."""
-        self.ctx.check(lib().lastro_kv8_evict(self.ctx.h, self._kv, dst._kv, _dev(lens), budget, recent, _dev(mass),
-                                              mass_stride, _dev(kept), _dev(lens_out), _dev(mass_out), mass_out_stride))
+        rc = self._evict(self.ctx.h, self._kv, dst._kv, _dev(lens), budget, recent, _dev(mass), mass_stride, _dev(kept),
+                         _dev(lens_out), _dev(mass_out), mass_out_stride)
+        if rc:
+            self.ctx.check(rc)
 
     def read(self, lens, pos0, n: int, k_out, v_out, dtype: str):
         """The values of slots [pos0[b], pos0[b] + n) of every sequence as bf16 or f32 (lastro_kv8_read)."""
         if dtype not in ("bf16", "f32"):
             raise LastroError(E_ARG, f"dtype {dtype!r} (bf16 or f32)")
-        self.ctx.check(lib().lastro_kv8_read(self.ctx.h, self._kv, _dev(lens), _dev(pos0), n, _dev(k_out), _dev(v_out),
-                                             _ROW_DTYPES[dtype]))
+        rc = self._read(self.ctx.h, self._kv, _dev(lens), _dev(pos0), n, _dev(k_out), _dev(v_out), _ROW_DTYPES[dtype])
+        if rc:
+            self.ctx.check(rc)
