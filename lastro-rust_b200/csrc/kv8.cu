@@ -412,7 +412,7 @@ LDEV uint32_t mul_f16(uint32_t x, uint32_t y) {
 constexpr int kGatherBlocks = 2;
 
 template <int FMT, int D>
-__global__ void __launch_bounds__(256) kv8_gather_kernel(const __grid_constant__ Kv8EvictArgs a) {
+__global__ void __launch_bounds__(256, D == 64 ? 4 : 2) kv8_gather_kernel(const __grid_constant__ Kv8EvictArgs a) {
     constexpr int LPR = D / 16, RPW = 32 / LPR, N = kKv8Block / RPW;  // lanes a row, rows a pass, passes
     static_assert(kGatherBlocks * kKv8Block == 32, "a lane for each row");
     pdl_wait();
