@@ -331,7 +331,8 @@ void lastro_batch_destroy(lastro_batch *batch);
  * Sequence lengths and row offsets are read on the device.  What the host cannot check there is checked by the kernels:
  * a page number outside the pool, a length outside the page table, row offsets outside the rows or beyond max_new make
  * the kernel skip that page or sequence and leave a LASTRO_KV8_BAD_* code in *status (device memory, may be NULL; never
- * cleared by the library).  Calls that share a cache, a workspace or outputs must not overlap on the GPU. */
+ * cleared by the library).  Slots, blocks and pages that hold no row may hold any bits; the e4m3 codes of NaN (0x7f, 0xff)
+ * are never written and are not looked for in rows.  Calls that share a cache, a workspace or outputs must not overlap on the GPU. */
 #define LASTRO_KV8_E4M3 1
 #define LASTRO_KV8_INT8 2
 #define LASTRO_KV8_PAGE 64
@@ -358,7 +359,7 @@ typedef struct {
 } lastro_rows;
 /* quantises new K and V rows into the cache: rows [new_off[b], new_off[b + 1]) (device, n_seqs + 1 offsets; at most
  * max_new rows a sequence) go to slots lens[b].. of sequence b, whose pages the page table already names.  A block that
- * holds earlier rows keeps its scale when the new ones fit it, else takes the larger scale and its codes are rounded to it.
+ * holds earlier rows keeps its scale when the new ones fit it (k and v have one dtype), else takes the larger scale and its codes are rounded to it.
  * Slots past the last row keep what they hold.  lens_out[b] = the new length (must not overlap lens); mass, when not
  * NULL, is the accumulated-weight array [n_seqs, kv_heads, mass_stride], whose new slots start at 0. */
 int lastro_kv8_append(lastro_ctx *ctx, const lastro_kv8 *kv, const int32_t *lens, const int32_t *new_off,
@@ -367,8 +368,8 @@ int lastro_kv8_append(lastro_ctx *ctx, const lastro_kv8 *kv, const int32_t *lens
 /* bytes of workspace lastro_kv8_attend needs for `heads` query heads and at most max_new queries a sequence */
 int lastro_kv8_attend_workspace(lastro_ctx *ctx, const lastro_kv8 *kv, int32_t heads, int32_t max_new,
                                 int32_t with_mass, size_t *bytes);
-/* grouped-query attention over the cache: rows [q_off[b], q_off[b + 1]) of q (heads a multiple of kv_heads) are the last
- * queries of sequence b, whose length lens[b] counts their own slots: query i of n sees slots [0, lens[b] - n + i].
+/* grouped-query attention over the cache: rows [q_off[b], q_off[b + 1]) of q (heads a multiple of kv_heads; at most
+ * n_seqs * max_new rows in all) are the last queries of sequence b, whose length lens[b] counts their own slots: query i of n sees slots [0, lens[b] - n + i].
  * out = softmax(scale * q k) v in q's dtype; a query that sees no slot gets zeros, one that holds a value that is not
  * finite gets NaN.  mass_out, when not NULL: [n_seqs, kv_heads, mass_stride] with mass_out[b, h, t] = mass_in[b, h, t] (0
  * when mass_in is NULL) + the attention weights slot t received from every query and every head of group h, for

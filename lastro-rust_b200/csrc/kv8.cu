@@ -21,14 +21,14 @@ __global__ void __launch_bounds__(256) kv8_append_kernel(const __grid_constant__
     if (j >= a.blocks) return;
     int64_t most = (int64_t)a.kv.max_pages * kKv8Page;
     if (a.mass) most = min(most, a.mass_stride);
-    const int len = seq_len(a.kv, a.lens, b, most);
+    const int given = __ldg(a.lens + b), len = seq_len(a.kv, a.lens, b, most);
     int first, n = seq_rows(a.kv, a.new_off, b, min(a.k.rows, a.v.rows), a.max_new, first);
-    if (n > most - len || __ldg(a.lens + b) != len) {
+    if (n > most - len || given != len) {
         if (n > most - len) report(a.kv, LASTRO_KV8_BAD_LENGTH);
         n = 0;
     }
     if (j == 0) {
-        if (h == 0 && lane == 0) a.lens_out[b] = len + n;
+        if (h == 0 && lane == 0) a.lens_out[b] = given + n;
         if (a.mass)
             for (int i = lane; i < n; i += 32) a.mass[((int64_t)b * H + h) * a.mass_stride + len + i] = 0.0f;
     }

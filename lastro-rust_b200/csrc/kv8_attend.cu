@@ -1214,7 +1214,7 @@ struct AttendLaunch {
             return kv8_launch<kv8_weights_kernel<D, F32>>(blocks, 128, 0, 1, s, a);
         }
         const int64_t rows = (int64_t)a.max_new * a.heads;
-        const dim3 grid((unsigned)min((int64_t)1024, (rows + kWarps - 1) / kWarps), a.kv.n_seqs);
+        const dim3 grid((unsigned)max((int64_t)1, min((int64_t)1024, (rows + kWarps - 1) / kWarps)), a.kv.n_seqs);
         e = kv8_launch<kv8_merge_kernel<D, FEW, RW, F32>>(grid, kThreads, 0, 1, s, a);
         if (e != cudaSuccess || !a.mass_out) return e;
         const int units = a.kv.kv_heads * a.kv.n_seqs, most = (a.kv.max_pages * (kKv8Page * D / kMassChunk) + kWarps - 1) / kWarps;

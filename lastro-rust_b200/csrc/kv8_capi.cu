@@ -67,6 +67,8 @@ extern "C" int lastro_kv8_append(lastro_ctx* ctx, const lastro_kv8* kv, const in
     KV8_TRY(check_rows(ctx, v, "kv8_append: v"));
     if (!lens || !new_off || !lens_out) return set_err(ctx, LASTRO_E_ARG, "kv8_append: null lens, new_off or lens_out");
     if (lens == lens_out) return set_err(ctx, LASTRO_E_ARG, "kv8_append: lens_out must not be lens");
+    if (misaligned(lens, 4) || misaligned(new_off, 4) || misaligned(lens_out, 4) || misaligned(mass, 4))
+        return set_err(ctx, LASTRO_E_ARG, "kv8_append: misaligned lens, new_off, lens_out or mass");
     if (k->dtype != v->dtype) return set_err(ctx, LASTRO_E_ARG, "kv8_append: k and v of different dtypes");
     if (max_new < 0) return set_err(ctx, LASTRO_E_ARG, "kv8_append: max_new %d", max_new);
     if (mass && mass_stride < 1) return set_err(ctx, LASTRO_E_ARG, "kv8_append: mass_stride %lld", (long long)mass_stride);
@@ -109,6 +111,8 @@ extern "C" int lastro_kv8_attend(lastro_ctx* ctx, const lastro_kv8* kv, const in
     KV8_TRY(check_rows(ctx, q, "kv8_attend: q"));
     KV8_TRY(check_rows(ctx, out, "kv8_attend: out"));
     if (!lens || !q_off || !workspace) return set_err(ctx, LASTRO_E_ARG, "kv8_attend: null lens, q_off or workspace");
+    if (misaligned(lens, 4) || misaligned(q_off, 4) || misaligned(mass_in, 4) || misaligned(mass_out, 4))
+        return set_err(ctx, LASTRO_E_ARG, "kv8_attend: misaligned lens, q_off or mass");
     if (heads < 1 || heads % kv->kv_heads)
         return set_err(ctx, LASTRO_E_ARG, "kv8_attend: %d heads for %d KV heads", heads, kv->kv_heads);
     if (max_new < 0) return set_err(ctx, LASTRO_E_ARG, "kv8_attend: max_new %d", max_new);
@@ -157,6 +161,8 @@ extern "C" int lastro_kv8_evict(lastro_ctx* ctx, const lastro_kv8* src, const la
         return set_err(ctx, LASTRO_E_ARG, "kv8_evict: src and dst differ in format, n_seqs, kv_heads or head_dim");
     if (!lens || !kept || !lens_out) return set_err(ctx, LASTRO_E_ARG, "kv8_evict: null lens, kept or lens_out");
     if (lens == lens_out) return set_err(ctx, LASTRO_E_ARG, "kv8_evict: lens_out must not be lens");
+    if (misaligned(lens, 4) || misaligned(kept, 4) || misaligned(lens_out, 4) || misaligned(mass, 4) || misaligned(mass_out, 4))
+        return set_err(ctx, LASTRO_E_ARG, "kv8_evict: misaligned lens, kept, lens_out or mass");
     if (budget < 1 || budget > (int64_t)dst->max_pages * kKv8Page)
         return set_err(ctx, LASTRO_E_ARG, "kv8_evict: budget %d (1 to the %lld slots of dst's page table)", budget,
                        (long long)dst->max_pages * kKv8Page);
@@ -191,6 +197,7 @@ extern "C" int lastro_kv8_read(lastro_ctx* ctx, const lastro_kv8* kv, const int3
     if (!lens || !pos0 || n < 0) return set_err(ctx, LASTRO_E_ARG, "kv8_read: null lens or pos0, or n %d", n);
     if (dtype != LASTRO_DTYPE_BF16 && dtype != LASTRO_DTYPE_F32)
         return set_err(ctx, LASTRO_E_ARG, "kv8_read: dtype %d (bf16 or f32)", dtype);
+    if (misaligned(lens, 4) || misaligned(pos0, 4)) return set_err(ctx, LASTRO_E_ARG, "kv8_read: misaligned lens or pos0");
     if (misaligned(k_out, 16) || misaligned(v_out, 16))
         return set_err(ctx, LASTRO_E_ARG, "kv8_read: outputs start on 16-byte boundaries");
     if (n == 0 || (!k_out && !v_out)) return LASTRO_OK;

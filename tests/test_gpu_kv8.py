@@ -697,6 +697,55 @@ def test_refusals(ctx):
     torch.cuda.synchronize()
 
 
+def test_misaligned_addresses_are_refused(ctx):
+    gpu, _, rng = filled(ctx, "e4m3", 1, 64, [20])
+    q, k = rows(rng, 1, 2, 64, "f32"), rows(rng, 1, 1, 64, "f32")
+    out, lens, off = torch.zeros_like(q), ints([20]), ints([0, 1])
+    n = gpu.c.attend_workspace(2, 1, True)
+    work, mass = torch.zeros(n, dtype=torch.uint8, device="cuda"), torch.zeros(1, 1, 64, device="cuda")
+    spare, kept = torch.zeros(1, dtype=torch.int32, device="cuda"), torch.zeros(1, 1, 16, dtype=torch.int32, device="cuda")
+    odd = lambda t: t.data_ptr() + 2  # noqa: E731
+    ro = LB.rows_of
+    att = dict(lens=lens, q_off=off, max_new=1, heads=2, q=ro(q), scale=0.1, out=ro(out), workspace=work, workspace_bytes=n,
+               mass_in=mass, mass_out=mass, mass_stride=64)
+    app = dict(lens=lens, new_off=off, max_new=1, k=ro(k), v=ro(k), lens_out=spare, mass=mass, mass_stride=64)
+    evi = dict(dst=gpu.c, lens=lens, budget=16, recent=4, mass=mass, mass_stride=64, kept=kept, lens_out=spare)
+    for f, args, names in ((gpu.c.attend, att, ("lens", "q_off", "mass_in", "mass_out")), (gpu.c.append, app, ("lens", "new_off", "lens_out", "mass")),
+                           (gpu.c.evict, evi, ("lens", "kept", "lens_out", "mass"))):
+        for name in names:
+            with pytest.raises(LB.LastroError) as e:
+                f(**(args | {name: odd(args[name])}))
+            assert e.value.code == LB.E_ARG
+    for a in ((odd(lens), lens), (lens, odd(lens))):
+        with pytest.raises(LB.LastroError):
+            gpu.c.read(*a, 1, k, None, "f32")
+    with pytest.raises(LB.LastroError):
+        gpu.c.append(**(app | dict(v=ro(k.bfloat16()))))
+
+
+def test_calls_without_rows(ctx):
+    """no query and no new row: lengths and masses are handed on"""
+    gpu, _, _ = filled(ctx, "int8", 2, 64, [70, 5])
+    n = gpu.c.attend_workspace(6, 0, True)
+    work, mass = torch.zeros(n, dtype=torch.uint8, device="cuda"), torch.rand(2, 2, 80, device="cuda")
+    out = torch.full_like(mass, -5.0)
+    r = LB.Rows(work.data_ptr(), LB.DTYPE_F32, 0, 64, 64)
+    gpu.c.attend(ints([70, 5]), ints([0, 0, 0]), 0, 6, r, 0.1, r, work, n, mass_in=mass, mass_out=out, mass_stride=80)
+    assert torch.equal(out[0, :, :70], mass[0, :, :70]) and torch.equal(out[1, :, :5], mass[1, :, :5])
+    assert (out[0, :, 70:] == -5.0).all() and (out[1, :, 5:] == -5.0).all()
+    for most in (0, 3, 40):  # room for queries, none there
+        n = gpu.c.attend_workspace(6, most, True)
+        work = torch.zeros(n, dtype=torch.uint8, device="cuda")
+        again = torch.full_like(mass, -5.0)
+        gpu.c.attend(ints([70, 5]), ints([0, 0, 0]), most, 6, r, 0.1, r, work, n, mass_in=mass, mass_out=again, mass_stride=80)
+        assert torch.equal(again, out)
+    lens = torch.zeros(2, dtype=torch.int32, device="cuda")
+    gpu.c.append(ints([70, 5]), ints([0, 0, 0]), 0, r, r, lens)
+    assert lens.tolist() == [70, 5] and gpu.status.item() == 0
+    gpu.c.append(ints([-3, 5]), ints([0, 0, 0]), 0, r, r, lens)
+    assert lens.tolist() == [-3, 5] and gpu.status.item() == LB.KV8_BAD_LENGTH
+
+
 def test_bad_device_data_is_reported_and_skipped(ctx):
     """page numbers outside the pool, lengths and offsets that do not fit: the other sequences' results stand"""
     lens, kv, d, heads = [100, 90, 30], 2, 64, 4
