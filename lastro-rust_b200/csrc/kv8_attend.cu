@@ -703,6 +703,10 @@ LDEV void store_merged(const Kv8AttendArgs& a, int first, int h, int r, const fl
 // A group of RW warps walks its part of the list through its own ring of stages, each a chunk of K and of V codes and
 // their scales brought in by bulk copies; its first warp's lane 0 issues them.  With one warp a group (RW 1) the CTA takes
 // one share, its warps equal parts of it in order, and puts together at its end what they cut.
+// Few rows are bound by memory: 254 us at 96 sequences of 7192 to 8192 slots with 32 heads of 128 (1.5 GB, 6.0 TB/s), 50 us at
+// 4 of 56537 to 65537 with 24 heads of 64 (5.3 TB/s).  Many rows are bound by the instructions that widen codes for each 16
+// rows: 28 us at 8 x 32 queries over 2048 slots (100 TFLOP/s).  A list too short for the card costs 7.5 us, of which 4.5 pass
+// before the first codes arrive (lengths, then page numbers, then copies).
 
 // what a warp of a CTA with one warp a group leaves behind
 struct Ends {
@@ -960,7 +964,8 @@ __global__ void __launch_bounds__(Shape<D, FEW, RW>::THREADS, 1) kv8_attend_kern
 }
 
 // ---- merging the shares -----------------------------------------------------------------------------------------------
-// One warp per query row and head whose unit was cut between shares, in the order of the shares.
+// One warp per query row and head whose unit was cut between shares, in the order of the shares.  3.3 us for a handful of rows
+// (three dependent loads), 7 us for 6144.
 template <int D, bool FEW, int RW, bool F32>
 __global__ void __launch_bounds__(kThreads) kv8_merge_kernel(const __grid_constant__ Kv8AttendArgs a) {
     using SH = Shape<D, FEW, RW>;
@@ -985,7 +990,8 @@ __global__ void __launch_bounds__(kThreads) kv8_merge_kernel(const __grid_consta
 // ---- accumulated weights, from stored scores ------------------------------------------------------------------------------
 // With few query rows the pass over the cache also leaves its scores (4 bytes a row and slot, against d bytes of K), and
 // the weights are one elementwise pass over them: a thread takes four slots.  The kernel merges the shares too: every CTA
-// needs the merged sums of its KV head's rows, and the head's first CTA their outputs.
+// needs the merged sums of its KV head's rows, and the head's first CTA their outputs.  13 us at 4 x 65537 slots, 8 KV heads and 3
+// rows (42 MB of scores and masses), 3.7 us where there is next to nothing to do.
 template <int D, bool F32>
 __global__ void __launch_bounds__(128) kv8_weights_kernel(const __grid_constant__ Kv8AttendArgs a) {
     using SH = Shape<D, true, 1>;
@@ -1052,7 +1058,8 @@ __global__ void __launch_bounds__(128) kv8_weights_kernel(const __grid_constant_
 // ---- accumulated weights, from K ------------------------------------------------------------------------------------------
 // More query rows: the scores are computed again, with the finished softmax sums at hand.  The chunks of each sequence and
 // KV head are dealt to the warps of gridDim.x CTAs; a warp holds a chunk's K in registers as f16 and runs the query tiles
-// past it from shared memory.  Two CTAs an SM, with half the chunk that one would take: latency is what bounds it.
+// past it from shared memory.  Two CTAs an SM, with half the chunk that one would take: latency is what bounds it (14 us at 8 x 32 queries over 2048
+// slots, 96 rows a KV head).
 constexpr int kMassTiles = kWarps, kMassChunk = 2048;  // query tiles in shared memory, one loaded by each warp; K codes a warp holds
 
 template <int D, bool F32>
