@@ -378,18 +378,7 @@ __global__ void __launch_bounds__(CL > 1 ? 1024 : 512) kv8_select_kernel(const _
     if (CL > 1) cluster_sync();  // no CTA leaves while another reads its counts
 }
 
-// four codes as two f16 pairs, exactly, and back (what they are multiplied by keeps them in the format's range)
-template <int FMT>
-LDEV void to_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
-    if (FMT == E4M3) {
-        asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(lo) : "h"((uint16_t)w));
-        asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(hi) : "h"((uint16_t)(w >> 16)));
-    } else {  // f16 0x6400 + u is 1024 + u for a byte u = code + 128
-        const uint32_t u = w ^ 0x80808080u, bias = 0x64806480u;
-        asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(lo) : "r"(__byte_perm(u, 0x64646464u, 0x4140)), "r"(bias));
-        asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(hi) : "r"(__byte_perm(u, 0x64646464u, 0x4342)), "r"(bias));
-    }
-}
+// and back: two f16 pairs to the nearest codes (what they were multiplied by keeps them in the format's range)
 template <int FMT>
 LDEV uint32_t from_f16(uint32_t lo, uint32_t hi) {
     if (FMT == E4M3) {
@@ -472,10 +461,10 @@ __global__ void __launch_bounds__(256, D == 64 ? 4 : 2) kv8_gather_kernel(const 
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 sc[i] = __shfl_sync(0xffffffffu, v ? vs : ks, g * kKv8Block + r0 + i * RPW);
-                to_f16<FMT>(w[g][v][i].x, f[i][0], f[i][1]);
-                to_f16<FMT>(w[g][v][i].y, f[i][2], f[i][3]);
-                to_f16<FMT>(w[g][v][i].z, f[i][4], f[i][5]);
-                to_f16<FMT>(w[g][v][i].w, f[i][6], f[i][7]);
+                widen<FMT>(w[g][v][i].x, f[i][0], f[i][1]);
+                widen<FMT>(w[g][v][i].y, f[i][2], f[i][3]);
+                widen<FMT>(w[g][v][i].z, f[i][4], f[i][5]);
+                widen<FMT>(w[g][v][i].w, f[i][6], f[i][7]);
                 uint32_t m = 0;  // magnitudes, ordered as their bits
 #pragma unroll
                 for (int q = 0; q < 8; ++q) m = __vmaxu2(m, f[i][q] & 0x7fff7fffu);

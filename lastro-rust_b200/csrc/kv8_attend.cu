@@ -53,20 +53,6 @@ LDEV float min_nan(float a, float b) {
     return y;
 }
 
-// four codes to two f16 pairs, exactly
-template <int FMT>
-LDEV void widen(uint32_t w, uint32_t& lo, uint32_t& hi) {
-    if (FMT == E4M3) {
-        asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(lo) : "h"((uint16_t)w));
-        asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(hi) : "h"((uint16_t)(w >> 16)));
-    } else {  // f16 0x6400 + u is 1024 + u for a byte u = code + 128
-        const uint32_t u = w ^ 0x80808080u, bias = 0x64806480u;  // 1152 twice
-        const uint32_t a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
-        asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(lo) : "r"(a), "r"(bias));
-        asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(hi) : "r"(b), "r"(bias));
-    }
-}
-
 LDEV uint32_t pack_f16(float lo, float hi) {
     uint32_t r;
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
