@@ -641,10 +641,10 @@ LDEV void add_parts(int n, At at, float (&o)[D / 32], float& M, float& R, float&
     const float old = pow2i(R - Rn), mine = pow2i(m.y - Rn);
 #pragma unroll
     for (int e = 0; e < V; ++e) o[e] *= old;
-    for (int i0 = 0; i0 < n; i0 += 8) {  // eight parts' loads on their way at a time
-        float x[8][V];
+    for (int i0 = 0; i0 < n; i0 += 4) {  // four parts' loads on their way at a time
+        float x[4][V];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < 4; ++i) {
 #pragma unroll
             for (int e = 0; e < V; ++e) x[i][e] = 0.0f;
             if (i0 + i < n) {
@@ -656,7 +656,7 @@ LDEV void add_parts(int n, At at, float (&o)[D / 32], float& M, float& R, float&
             }
         }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < 4; ++i) {
             const float f = __shfl_sync(0xffffffffu, mine, i0 + i);
 #pragma unroll
             for (int e = 0; e < V; ++e)
@@ -951,7 +951,7 @@ __global__ void __launch_bounds__(Shape<D, FEW, RW>::THREADS, 1) kv8_attend_kern
 
 // ---- merging the shares -----------------------------------------------------------------------------------------------
 // One warp per query row and head whose unit was cut between shares, in the order of the shares.  3.3 us for a handful of rows
-// (three dependent loads), 7 us for 6144.
+// (three dependent loads), 5.6 us for 6144.
 template <int D, bool FEW, int RW, bool F32>
 __global__ void __launch_bounds__(kThreads) kv8_merge_kernel(const __grid_constant__ Kv8AttendArgs a) {
     using SH = Shape<D, FEW, RW>;
