@@ -1,5 +1,5 @@
 // Attention over the 8-bit KV cache (lastro_kv8_attend): scores, softmax and weighted sum in one pass over the cache, the
-// weights every slot received in a second pass over K.
+// weights every slot received in a second pass over the scores it kept, or over K.
 //
 // A KV head's query rows are its group's heads times the sequence's queries.  The products are m16n8k16 matrix products,
 // a block's 16 slots at a time, in one of two forms:
@@ -18,7 +18,7 @@ namespace lastro {
 namespace {
 
 constexpr int kWarps = 8, kThreads = kWarps * 32;  // of the merge and mass kernels
-constexpr float kFar = -1e30f;                        // below every score: the running maxima's start
+constexpr float kFar = -1e30f;                    // below every score: the running maxima's start
 
 LDEV float ex2(float x) {
     float y;
@@ -96,9 +96,9 @@ LDEV int slot_of(int pair, int e, int j) { return j * 8 + e * 4 + (pair & 2) + (
 template <int D, bool FEW, int RW>
 struct Shape {
     static constexpr int WARPS = 8, THREADS = WARPS * 32, GROUPS = WARPS / RW;
-    static constexpr int ROWS = FEW ? 8 : 16, TILE = RW * ROWS;     // query rows of a warp and of a unit
-    static constexpr int CHUNK = 4096, TOK = CHUNK / D; // K (or V) codes and slots of a stage
-    static constexpr int NB = TOK / kKv8Block, CPP = kKv8Page / TOK; // blocks of a chunk, chunks of a page
+    static constexpr int ROWS = FEW ? 8 : 16, TILE = RW * ROWS;       // query rows of a warp and of a unit
+    static constexpr int CHUNK = 4096, TOK = CHUNK / D;               // K (or V) codes and slots of a stage
+    static constexpr int NB = TOK / kKv8Block, CPP = kKv8Page / TOK;  // blocks of a chunk, chunks of a page
     static constexpr int STAGES = FEW ? 3 : RW == 1 ? 2 : 6;
     static constexpr int PART = D + 4;  // floats of one row's partial result: its sums, then M, R and l
     // items of a share: a chunk for each warp, and of groups enough that merging does not cost more than they do (one
