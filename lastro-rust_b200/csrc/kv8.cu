@@ -33,8 +33,9 @@ __global__ void __launch_bounds__(256) kv8_append_kernel(const __grid_constant__
         if (a.mass)
             for (int i = lane; i < n; i += 32) a.mass[((int64_t)b * H + h) * a.mass_stride + len + i] = 0.0f;
     }
-    const int slot0 = (len / kKv8Block + j) * kKv8Block;  // the block's first slot
-    if (n == 0 || slot0 >= len + n) return;
+    const int tail = len % kKv8Block;  // earlier rows of the first block
+    if (n == 0 || j * kKv8Block >= tail + n) return;
+    const int slot0 = len - tail + j * kKv8Block;  // the block's first slot
     const int page = page_of(a.kv, b, slot0);
     if (page < 0) return;
     const int beg = max(0, len - slot0), end = min(kKv8Block, len + n - slot0);  // its new rows

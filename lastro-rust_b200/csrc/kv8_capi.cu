@@ -1,4 +1,5 @@
 // C ABI of the 8-bit KV cache: argument checks and launches (lastro_kv8_* in include/lastro_b200.h).
+#include <algorithm>
 #include <cmath>
 
 #include "capi_internal.h"
@@ -78,14 +79,15 @@ extern "C" int lastro_kv8_append(lastro_ctx* ctx, const lastro_kv8* kv, const in
     a.new_off = new_off;
     a.k = *k;
     a.v = *v;
-    // rows beyond the page table are refused on the device, so no sequence takes more
-    a.max_new = (int32_t)std::min<int64_t>(max_new, (int64_t)kv->max_pages * kKv8Page);
+    // rows beyond the page table are refused on the device, so no sequence takes more, nor more than there are
+    a.max_new = (int32_t)std::min({(int64_t)max_new, (int64_t)kv->max_pages * kKv8Page, (int64_t)std::min(k->rows, v->rows)});
     a.blocks = a.max_new ? (a.max_new + 2 * kKv8Block - 2) / kKv8Block : 1;
     a.lens_out = lens_out;
     a.mass = mass;
     a.mass_stride = mass_stride;
-    if ((int64_t)kv->n_seqs * a.blocks * kv->kv_heads * 2 / 8 >= INT32_MAX)
-        return set_err(ctx, LASTRO_E_UNSUPPORTED, "kv8_append: n_seqs %d with max_new %d in one call", kv->n_seqs, max_new);
+    if ((int64_t)a.blocks * kv->kv_heads > INT32_MAX - 7)  // blocks and heads of a sequence, eight to a CTA, counted in 32 bits
+        return set_err(ctx, LASTRO_E_UNSUPPORTED, "kv8_append: %d rows of %d KV heads to a sequence in one call", a.max_new,
+                       kv->kv_heads);
     KV8_TRY(on_device(ctx, "kv8_append"));
     return launched(ctx, launch_kv8_append(a, ctx->stream), "kv8_append");
 }
@@ -184,8 +186,6 @@ extern "C" int lastro_kv8_evict(lastro_ctx* ctx, const lastro_kv8* src, const la
     a.lens_out = lens_out;
     a.mass_out = mass_out;
     a.mass_out_stride = mass_out_stride;
-    if ((int64_t)src->n_seqs * src->kv_heads * ((budget + kKv8Block - 1) / kKv8Block) * 2 / 8 >= INT32_MAX)
-        return set_err(ctx, LASTRO_E_UNSUPPORTED, "kv8_evict: n_seqs %d with budget %d in one call", src->n_seqs, budget);
     KV8_TRY(on_device(ctx, "kv8_evict"));
     return launched(ctx, launch_kv8_evict(a, ctx->stream), "kv8_evict");
 }
