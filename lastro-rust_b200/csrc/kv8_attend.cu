@@ -195,6 +195,8 @@ LDEV void find_part(int* room, int n_seqs, Work work, Part part, Note note, int&
             }
         sum += here;
     }
+    // `room` is in the rings: its ordinary accesses before the bulk copies to come, which write through another proxy
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncthreads();
 }
 

@@ -46,3 +46,17 @@ def test_append_of_more_rows_than_can_be_counted_is_refused(ctx):
     assert code_of(c.append, ints([0]), ints([0, 1]), 1 << 30, one, one, out) == LB.E_UNSUPPORTED
     torch.cuda.synchronize()
     assert gpu.status.item() == 0
+
+
+# ---- shared memory ------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("news", [1, 12])
+def test_copies_that_follow_the_list_closely(ctx, news):
+    """many short sequences: the list is written several times over where the first copies go; every repeat gives the same"""
+    lens = (np.arange(1500) * 7 % 61 + 12).tolist()
+    gpu, ref, rng = filled(ctx, "int8", 1, 64, lens)
+    check_attend(gpu, ref, rng, lens, [news] * len(lens), 2, "bf16")
+    q = [rows(rng, news, 2, 64, "bf16") for _ in lens]
+    first = gpu.attend(lens, q, 0.125, mass=True)
+    for _ in range(30):
+        again = gpu.attend(lens, q, 0.125, mass=True)
+        assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
