@@ -22,7 +22,7 @@ __global__ void __launch_bounds__(256) kv8_append_kernel(const __grid_constant__
     if (j >= a.blocks) return;
     int64_t most = (int64_t)a.kv.max_pages * kKv8Page;
     if (a.mass) most = min(most, a.mass_stride);
-    const int given = __ldg(a.lens + b), len = seq_len(a.kv, a.lens, b, most);
+    const int given = a.lens[b], len = seq_len(a.kv, a.lens, b, most);
     int first, n = seq_rows(a.kv, a.new_off, b, min(a.k.rows, a.v.rows), a.max_new, first);
     if (n > most - len || given != len) {
         if (n > most - len) report(a.kv, LASTRO_KV8_BAD_LENGTH);
@@ -117,7 +117,7 @@ __global__ void __launch_bounds__(256, 5) kv8_read_kernel(const __grid_constant_
     const int j0 = (blockIdx.x * 8 + (threadIdx.x >> 5)) * kReadSlots;
     if (j0 >= a.n) return;
     const int len = seq_len(a.kv, a.lens, b, (int64_t)a.kv.max_pages * kKv8Page);
-    const int64_t pos0 = (int64_t)__ldg(a.pos0 + b) + j0;
+    const int64_t pos0 = (int64_t)a.pos0[b] + j0;
     int page[kReadSlots];
 #pragma unroll
     for (int i = 0; i < kReadSlots; ++i)
@@ -136,8 +136,8 @@ __global__ void __launch_bounds__(256, 5) kv8_read_kernel(const __grid_constant_
                 w[v][i] = make_uint2(0, 0);
                 s[v][i] = 0.0f;
                 if (page[i] >= 0 && (v ? a.v_out : a.k_out)) {
-                    w[v][i] = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(v ? a.kv.v : a.kv.k) + (tile * kKv8Page + row) * D + c));
-                    s[v][i] = __ldg((v ? a.kv.v_scale : a.kv.k_scale) + tile * kKv8Blocks + row / kKv8Block);
+                    w[v][i] = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(v ? a.kv.v : a.kv.k) + (tile * kKv8Page + row) * D + c);
+                    s[v][i] = (v ? a.kv.v_scale : a.kv.k_scale)[tile * kKv8Blocks + row / kKv8Block];
                 }
             }
         }
@@ -244,12 +244,12 @@ __global__ void __launch_bounds__(CL > 1 ? 1024 : 512) kv8_select_kernel(const _
     auto fetch = [&](int i) {
         const float* p = mass + lo + 4 * i;
         if (vec && 4 * i + 4 <= n) {
-            const float4 m = __ldg(reinterpret_cast<const float4*>(p));
+            const float4 m = *reinterpret_cast<const float4*>(p);
             return make_uint4(mass_key(m.x), mass_key(m.y), mass_key(m.z), mass_key(m.w));
         }
         uint32_t k[4];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) k[q] = 4 * i + q < n ? mass_key(__ldg(p + q)) : 0u;
+        for (int q = 0; q < 4; ++q) k[q] = 4 * i + q < n ? mass_key(p[q]) : 0u;
         return make_uint4(k[0], k[1], k[2], k[3]);
     };
     if (held) {
@@ -402,7 +402,7 @@ LDEV uint32_t mul_f16(uint32_t x, uint32_t y) {
 // 16 bytes of a row whose neighbours are as likely dropped as kept: no more than its 64 bytes are fetched
 LDEV uint4 ld_row(const uint8_t* p) {
     uint4 r;
-    asm("ld.global.nc.L1::no_allocate.L2::64B.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
+    asm volatile("ld.global.L1::no_allocate.L2::64B.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p) : "memory");
     return r;
 }
 
@@ -421,19 +421,19 @@ __global__ void __launch_bounds__(256, D == 64 ? 4 : 2) kv8_gather_kernel(const 
     pdl_launch();
     const int lane = threadIdx.x & 31, H = a.src.kv_heads, h = blockIdx.y, b = blockIdx.z;
     const int slot0 = (blockIdx.x * 8 + (threadIdx.x >> 5)) * 32;
-    const int keep = __ldcg(a.lens_out + b);
+    const int keep = a.lens_out[b];
     if (slot0 >= keep) return;
     const int dpage = page_of(a.dst, b, slot0);  // both blocks are in one page
     // lane r: where kept row r is, and its scales
     int64_t from = -1;
     float ks = 0.0f, vs = 0.0f;
     if (slot0 + lane < keep) {
-        const int t = __ldcg(a.kept + ((int64_t)b * H + h) * a.budget + slot0 + lane), page = page_of(a.src, b, t);
+        const int t = a.kept[((int64_t)b * H + h) * a.budget + slot0 + lane], page = page_of(a.src, b, t);
         if (page >= 0) {
             const int64_t tile = (int64_t)page * H + h;
             from = tile * kKv8Page + t % kKv8Page;
-            ks = __ldg(a.src.k_scale + tile * kKv8Blocks + t % kKv8Page / kKv8Block);
-            vs = __ldg(a.src.v_scale + tile * kKv8Blocks + t % kKv8Page / kKv8Block);
+            ks = a.src.k_scale[tile * kKv8Blocks + t % kKv8Page / kKv8Block];
+            vs = a.src.v_scale[tile * kKv8Blocks + t % kKv8Page / kKv8Block];
         }
     }
     if (dpage < 0) return;

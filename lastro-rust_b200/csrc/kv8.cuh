@@ -13,13 +13,16 @@ namespace lastro {
 constexpr int E4M3 = LASTRO_KV8_E4M3, INT8 = LASTRO_KV8_INT8;
 
 // ---- checks on device data ------------------------------------------------------------------------------------------
+// Lengths, tables, rows, codes, scales and masses are what earlier calls on the stream, or the program between them, left
+// behind, and these kernels are resident before that has ended: they are read with ordinary loads, which stay behind
+// pdl_wait() and see what it waited for.  (The read-only path promises neither.)
 LDEV void report(const lastro_kv8& kv, int code) {
     if (kv.status) atomicExch(kv.status, code);
 }
 
 // the page of slot `slot` of sequence b, or -1
 LDEV int page_of(const lastro_kv8& kv, int b, int slot) {
-    const int p = __ldg(kv.page_table + (int64_t)b * kv.max_pages + slot / kKv8Page);
+    const int p = kv.page_table[(int64_t)b * kv.max_pages + slot / kKv8Page];
     if ((unsigned)p < (unsigned)kv.num_pages) return p;
     report(kv, LASTRO_KV8_BAD_PAGE);
     return -1;
@@ -27,7 +30,7 @@ LDEV int page_of(const lastro_kv8& kv, int b, int slot) {
 
 // a sequence's length, 0 when it is not one the page table (or `most` slots) can hold
 LDEV int seq_len(const lastro_kv8& kv, const int32_t* lens, int b, int64_t most) {
-    const int n = __ldg(lens + b);
+    const int n = lens[b];
     if (n >= 0 && n <= most) return n;
     report(kv, LASTRO_KV8_BAD_LENGTH);
     return 0;
@@ -35,8 +38,8 @@ LDEV int seq_len(const lastro_kv8& kv, const int32_t* lens, int b, int64_t most)
 
 // rows of sequence b: first row, and their number (0 when the offsets are not usable)
 LDEV int seq_rows(const lastro_kv8& kv, const int32_t* off, int b, int rows, int max_new, int& first) {
-    first = __ldg(off + b);
-    const int end = __ldg(off + b + 1);
+    first = off[b];
+    const int end = off[b + 1];
     if (first >= 0 && end >= first && end <= rows && end - first <= max_new) return end - first;
     report(kv, LASTRO_KV8_BAD_OFFSET);
     return 0;
@@ -108,16 +111,16 @@ struct Raw8 {
         if (vec) {
 #pragma unroll
             for (int i = 0; i < (F32 ? 2 : 1); ++i) {
-                const uint4 v = __ldg(reinterpret_cast<const uint4*>(p) + i);
+                const uint4 v = reinterpret_cast<const uint4*>(p)[i];
                 w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
             }
         } else if (F32) {
 #pragma unroll
-            for (int i = 0; i < (F32 ? 8 : 4); ++i) w[i] = __ldg(reinterpret_cast<const uint32_t*>(p) + i);
+            for (int i = 0; i < (F32 ? 8 : 4); ++i) w[i] = reinterpret_cast<const uint32_t*>(p)[i];
         } else {
             const uint16_t* q = reinterpret_cast<const uint16_t*>(p);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) w[i] = __ldg(q + 2 * i) | (uint32_t)__ldg(q + 2 * i + 1) << 16;
+            for (int i = 0; i < 4; ++i) w[i] = q[2 * i] | (uint32_t)q[2 * i + 1] << 16;
         }
     }
     LDEV void zero() {

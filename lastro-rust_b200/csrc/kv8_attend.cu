@@ -795,7 +795,7 @@ __global__ void __launch_bounds__(Shape<D, FEW, RW>::THREADS, 1) kv8_attend_kern
             if (iss.b != pb || pg < pbase || pg >= pbase + 32) {
                 pb = iss.b, pbase = pg;
                 const int pages = (iss.s.len + kKv8Page - 1) / kKv8Page;
-                pnum = pg + lane < pages ? __ldg(a.kv.page_table + (int64_t)pb * a.kv.max_pages + pg + lane) : -1;
+                pnum = pg + lane < pages ? a.kv.page_table[(int64_t)pb * a.kv.max_pages + pg + lane] : -1;
             }
             const int page = __shfl_sync(0xffffffffu, pnum, pg - pbase);
             if (lane == 0) {
@@ -994,7 +994,7 @@ __global__ void __launch_bounds__(128) kv8_weights_kernel(const __grid_constant_
     for (int r = threadIdx.x >> 5; r < rows; r += 4) {
         if (g0 == g1) {
             const int i = query_of(r, a.group);
-            if (lane == 0) sums[r] = __ldcg(a.lse + (int64_t)(s.first + i) * a.heads + h * a.group + r - i * a.group);
+            if (lane == 0) sums[r] = a.lse[(int64_t)(s.first + i) * a.heads + h * a.group + r - i * a.group];
             continue;
         }
         const auto part = [&](int g) { return a.part + (((int64_t)g * 2 + (g == g0)) * SH::TILE + r) * SH::PART; };
@@ -1027,7 +1027,7 @@ __global__ void __launch_bounds__(128) kv8_weights_kernel(const __grid_constant_
 #pragma unroll
             for (int r = 0; r < 8; ++r)
                 if (r < rows) {
-                    const float4 v = __ldcg(reinterpret_cast<const float4*>(src + r * SH::TOK));
+                    const float4 v = *reinterpret_cast<const float4*>(src + r * SH::TOK);
                     sum[0] += ex2(v.x - lse[r]), sum[1] += ex2(v.y - lse[r]);
                     sum[2] += ex2(v.z - lse[r]), sum[3] += ex2(v.w - lse[r]);
                 }
@@ -1085,7 +1085,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv8_mass_kernel(const __grid_cons
             const uint8_t* kp = static_cast<const uint8_t*>(a.kv.k) + tile * kKv8Page * D + (int64_t)(c % CPP) * kMassChunk;
 #pragma unroll
             for (int n = 0; n < NB; ++n) {
-                ks_next[n] = __ldg(a.kv.k_scale + tile * kKv8Blocks + (c % CPP) * NB + n);
+                ks_next[n] = a.kv.k_scale[tile * kKv8Blocks + (c % CPP) * NB + n];
 #pragma unroll
                 for (int j = 0; j < 2; ++j) k_codes<D>(kp + (n * 16 + slot_of(gq >> 1, gq & 1, j)) * D, w[n][j]);
             }
@@ -1110,7 +1110,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv8_mass_kernel(const __grid_cons
                     const int r = row0 + gq + 8 * e, at = warp * 16 + gq + 8 * e, i = r / a.group;
                     rfac[at] = q.factor[e];
                     rvis[at] = visible(a, s, r);
-                    rlse[at] = r < rows ? __ldcg(a.lse + (int64_t)(s.first + i) * a.heads + h * a.group + r - i * a.group) : INFINITY;
+                    rlse[at] = r < rows ? a.lse[(int64_t)(s.first + i) * a.heads + h * a.group + r - i * a.group] : INFINITY;
                 }
         }
         __syncthreads();

@@ -60,3 +60,52 @@ def test_copies_that_follow_the_list_closely(ctx, news):
     for _ in range(30):
         again = gpu.attend(lens, q, 0.125, mass=True)
         assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
+
+
+# ---- calls right behind one another ---------------------------------------------------------------------------------------
+@pytest.mark.parametrize("fmt,dtype,new", [("e4m3", "bf16", 1), ("int8", "f32", 6)])
+def test_a_chain_of_calls_passes_its_results_on_the_device(ctx, fmt, dtype, new):
+    """append, attend, evict, read, with lengths, masses and kept slots that stay on the device and nothing between the
+    launches; again and again over the same buffers"""
+    kv, d, heads, budget, recent, room = 2, 64, 4, 40, 8, 128
+    lens = [100, 57, 41, 3]
+    rng = np.random.default_rng(21)
+    src, dst = Gpu(ctx, fmt, 4, kv, d, 2), Gpu(ctx, fmt, 4, kv, d, 1, seed=5)
+    first = [[rows(rng, n, kv, d, dtype) for n in lens] for _ in "kv"]
+    off0, off = ints(np.concatenate([[0], np.cumsum(lens)]).tolist()), ints([new * i for i in range(5)])
+    zero, l0, l1, l2 = ints([0] * 4), ints([-1] * 4), ints([-1] * 4), ints([-1] * 4)
+    mass, mass2 = (torch.zeros(4, kv, n, device="cuda") for n in (room, budget))
+    kept = torch.zeros(4, kv, budget, dtype=torch.int32, device="cuda")
+    out = torch.zeros(4 * new, heads, d, dtype=torch.bfloat16 if dtype == "bf16" else torch.float32, device="cuda")
+    k, v = (torch.zeros(4, budget, kv, d, device="cuda") for _ in "kv")
+    work = torch.zeros(src.c.attend_workspace(heads, new, True), dtype=torch.uint8, device="cuda")
+    keep_alive = [torch.cat(x) for x in first]
+    all0 = [LB.rows_of(x) for x in keep_alive]
+    for step in range(8):
+        q = [rows(rng, new, heads, d, dtype) for _ in lens]
+        kn, vn = ([rows(rng, new, kv, d, dtype) for _ in lens] for _ in "kv")
+        qc, kc, vc = (torch.cat(x) for x in (q, kn, vn))
+        torch.cuda.synchronize()
+        src.c.append(zero, off0, max(lens), *all0, l0, mass, room)
+        src.c.append(l0, off, new, LB.rows_of(kc), LB.rows_of(vc), l1, mass, room)
+        src.c.attend(l1, off, new, heads, LB.rows_of(qc), 0.125, LB.rows_of(out), work, work.numel(), mass_in=mass, mass_out=mass,
+                     mass_stride=room)
+        src.c.evict(dst.c, l1, budget, recent, mass, room, kept, l2, mass2, budget)
+        dst.c.read(l2, zero, budget, k, v, "f32")
+        ref = R.Cache(4, kv, d, fmt)
+        got, gm, at = f64(out), f64(mass), 0
+        assert l1.tolist() == [n + new for n in lens] and l2.tolist() == [min(n + new, budget) for n in lens]
+        for b, n in enumerate(lens):
+            ref.append(b, f64(first[0][b]), f64(first[1][b]))
+            ref.append(b, f64(kn[b]), f64(vn[b]))
+            want, wm, big = ref.attend(b, f64(q[b]), 0.125)
+            vmax = max(np.abs(ref.side[b][h]["v"].values()).max() for h in range(kv))
+            rel, tol = bounds(dtype, d, big, vmax)
+            assert (np.abs(got[at:at + new] - want) <= tol + (2.0 ** -8 * np.abs(want) if dtype == "bf16" else 0.0)).all()
+            assert (np.abs(gm[b, :, :n + new] - wm) <= rel * wm + 2.0 ** -22 * wm).all()
+            at += new
+            for h, keep in enumerate(ref.evict(b, gm[b, :, :n + new], budget, recent)):
+                assert kept[b, h, :len(keep)].tolist() == keep.tolist()
+                for w, x in (("k", k), ("v", v)):
+                    assert np.array_equal(f64(x[b, :len(keep), h]), ref.side[b][h][w].values())
+    assert src.status.item() == 0 and dst.status.item() == 0
