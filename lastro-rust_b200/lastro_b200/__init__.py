@@ -59,9 +59,10 @@ class Kv8Desc(C.Structure):
 
 
 class Rows(C.Structure):
-    """lastro_rows: activation rows [rows, heads, head_dim] on the device, strides in elements."""
+    """lastro_rows: activation rows [rows, heads, head_dim] on the device, strides in elements.  The last field is this
+    binding's own: heads << 33 | head_dim << 2 | on the GPU << 1 | 1 as rows_of saw them, which the calls hold against theirs, or 0."""
     _fields_ = [("ptr", C.c_void_p), ("dtype", C.c_int32), ("rows", C.c_int32), ("row_stride", C.c_int64),
-                ("head_stride", C.c_int64)]
+                ("head_stride", C.c_int64), ("shape", C.c_int64)]
 
 
 EXPORTS = {
@@ -803,9 +804,59 @@ _ROW_DTYPES = {"torch.bfloat16": DTYPE_BF16, "torch.float32": DTYPE_F32, "bf16":
 _row_dtypes = {}  # the same by the dtype objects met so far
 
 
-def _dev(x):
-    """A device address: an int, None, or anything with data_ptr() (a torch tensor)."""
-    return x if x is None or x.__class__ is int else x.data_ptr()
+_INT32 = _FLOAT32 = _BF16 = None  # torch's types, once there are tensors (torch itself is not imported here)
+
+
+def _learn() -> bool:
+    global _INT32, _FLOAT32, _BF16
+    torch = sys.modules.get("torch")
+    if torch is None or _INT32 is not None:
+        return False
+    _INT32, _FLOAT32, _BF16 = torch.int32, torch.float32, torch.bfloat16
+    return True
+
+
+def _unfit(x, what: str, want: str):
+    return LastroError(E_ARG, f"kv8_{what}: {want} on the GPU wanted, not {tuple(x.shape)} {x.dtype} with strides {x.stride()} "
+                              f"on {x.device}")
+
+
+# Device addresses from ints and None, which cannot be checked, and from tensors, which are.  A call of a few microseconds is
+# made several times a layer: what is as it should be takes as few steps as there are (0.2 us a tensor).
+def _ints(x, nbytes: int, what: str):
+    """dense int32"""
+    if x.__class__ is int or x is None:
+        return x
+    if x.dtype is _INT32 and x.nbytes >= nbytes and x.is_cuda and x.is_contiguous():
+        return x.data_ptr()
+    if _learn():
+        return _ints(x, nbytes, what)
+    raise _unfit(x, what, f"dense torch.int32 of {nbytes} bytes")
+
+
+def _dense(x, nbytes: int, what: str, dtype=None):
+    """dense, of type `dtype` or any"""
+    if x.__class__ is int or x is None:
+        return x
+    if (dtype is None or x.dtype is dtype) and x.nbytes >= nbytes and x.is_cuda and x.is_contiguous():
+        return x.data_ptr()
+    raise _unfit(x, what, f"dense {dtype or 'tensor'} of {nbytes} bytes")
+
+
+def _masses(x, n_seqs: int, kv_heads: int, stride: int, what: str):
+    """f32 masses [n_seqs, kv_heads, stride]: dense, or the first columns of rows that long"""
+    if x.__class__ is int or x is None:
+        return x
+    if x.ndim != 3:
+        return _dense(x, 4 * n_seqs * kv_heads * stride, what, _FLOAT32)
+    (s0, s1, s2), (n, heads, cols) = x.stride(), x.shape
+    if x.dtype is not _FLOAT32 or not x.is_cuda or s2 != 1 or n < n_seqs or heads != kv_heads or (s1 != stride and heads > 1) or \
+            (s0 != heads * stride and n_seqs > 1) or \
+            (cols < stride and x.untyped_storage().nbytes() < 4 * (x.storage_offset() + n_seqs * heads * stride)):
+        if _learn():
+            return _masses(x, n_seqs, kv_heads, stride, what)
+        raise _unfit(x, what, f"torch.float32 [{n_seqs}, {kv_heads}, ..] in rows of {stride}")
+    return x.data_ptr()
 
 
 def rows_of(t) -> Rows:
@@ -816,7 +867,8 @@ def rows_of(t) -> Rows:
         dtype = _row_dtypes[t.dtype] = _ROW_DTYPES.get(str(t.dtype), 0)
     if not dtype or len(strides) != 3 or strides[2] != 1:
         raise LastroError(E_ARG, f"rows: {tuple(t.shape)} {t.dtype} with strides {strides} (bf16 or f32, last axis dense)")
-    return Rows(t.data_ptr(), dtype, t.shape[0], strides[0], strides[1])
+    rows, heads, dim = t.shape
+    return Rows(t.data_ptr(), dtype, rows, strides[0], strides[1], heads << 33 | dim << 2 | (3 if t.is_cuda else 1))
 
 
 class Kv8Cache:
@@ -825,8 +877,9 @@ class Kv8Cache:
     The caller owns the device buffers (addresses as ints, or torch tensors): k, v codes [num_pages, kv_heads, 64,
     head_dim] bytes, k_scale, v_scale [num_pages, kv_heads, 4] f32, page_table [n_seqs, max_pages] int32, status one int32
     word or None (a KV8_BAD_* code when a kernel met a page, length or offset it could not use).  Arguments named lens,
-    new_off, q_off, pos0, lens_out and kept are int32 on the device, mass arrays f32.  Every call enqueues on the
-    context's stream and returns; tensors passed in are not kept alive by it."""
+    new_off, q_off, pos0, lens_out and kept are int32 on the device, mass arrays f32.  Tensors are held against what a call
+    will read and write of them (type, place, layout, size), addresses cannot be.  Every call enqueues on the context's
+    stream and returns; tensors passed in are not kept alive by it."""
 
     def __init__(self, ctx: Context, fmt: str, n_seqs: int, kv_heads: int, head_dim: int, num_pages: int, max_pages: int,
                  k, v, k_scale, v_scale, page_table, status=None):
@@ -834,19 +887,38 @@ class Kv8Cache:
             raise LastroError(E_ARG, f"format {fmt!r} (one of {', '.join(KV8_FORMATS)})")
         self.ctx = ctx
         self.buffers = (k, v, k_scale, v_scale, page_table, status)  # tensors live as long as the cache
+        # sizes that the calls refuse say nothing about what the buffers should hold
+        self._sized = head_dim in (64, 128) and min(n_seqs, kv_heads, num_pages, max_pages) > 0 and max_pages <= 1 << 24
+        codes, scales = (num_pages * kv_heads * n for n in (KV8_PAGE * head_dim, KV8_PAGE // KV8_BLOCK * 4))
+        want = (codes, codes, scales, scales, n_seqs * max_pages * 4, 4) if self._sized else (0,) * 6
+        _learn()
+        types = (None, None, _FLOAT32, _FLOAT32, _INT32, _INT32)
+        names = ("k", "v", "k_scale", "v_scale", "page_table", "status")
         self.desc = Kv8Desc(KV8_FORMATS[fmt], n_seqs, kv_heads, head_dim, num_pages, max_pages,
-                            *(_dev(x) for x in self.buffers))
+                            *(_dense(x, n, "cache: " + w, t) for x, n, w, t in zip(self.buffers, want, names, types)))
+        self._lens, self._seqs, self._heads, self._dim, self._rows = 4 * n_seqs, n_seqs, kv_heads, head_dim, kv_heads << 33 | head_dim << 2 | 3
+        self._slot = n_seqs * kv_heads * head_dim * 2 if self._sized else 0  # bytes of one slot of every sequence in bf16
         # what a call of a few microseconds should not look up again
         L = lib()
         self._kv = C.byref(self.desc)
         self._append, self._attend, self._evict, self._read = (L.lastro_kv8_append, L.lastro_kv8_attend, L.lastro_kv8_evict,
                                                                L.lastro_kv8_read)
 
+    def _check_rows(self, what: str, rows, want: int):
+        for r in rows:
+            if r.shape not in (0, want) and self._sized:
+                raise LastroError(E_ARG, f"kv8_{what}: rows of {r.shape >> 33} heads of {r.shape >> 2 & 0x7fffffff} on the "
+                                         f"{'GPU' if r.shape & 2 else 'host'}, {want >> 33} of {self._dim} on the GPU wanted")
+
     def append(self, lens, new_off, max_new: int, k: Rows, v: Rows, lens_out, mass=None, mass_stride: int = 0):
         """Quantise rows [new_off[b], new_off[b + 1]) of k and v into slots lens[b].. of each sequence
         (lastro_kv8_append)."""
-        rc = self._append(self.ctx.h, self._kv, _dev(lens), _dev(new_off), max_new, k, v, _dev(lens_out), _dev(mass),
-                          mass_stride)
+        n, rows = self._lens, self._rows
+        if k.shape != rows or v.shape != rows:
+            self._check_rows("append", (k, v), rows)
+        rc = self._append(self.ctx.h, self._kv, _ints(lens, n, "append: lens"), _ints(new_off, n + 4, "append: new_off"),
+                          max_new, k, v, _ints(lens_out, n, "append: lens_out"),
+                          _masses(mass, self._seqs, self._heads, mass_stride, "append: mass"), mass_stride)
         if rc:
             self.ctx.check(rc)
 
@@ -861,8 +933,14 @@ class Kv8Cache:
                workspace_bytes: int, mass_in=None, mass_out=None, mass_stride: int = 0):
         """out = softmax(scale * q k) v over the slots each query sees; mass_out = mass_in + the weights each slot
         received (lastro_kv8_attend)."""
-        rc = self._attend(self.ctx.h, self._kv, _dev(lens), _dev(q_off), max_new, heads, q, scale, out, _dev(mass_in),
-                          _dev(mass_out), mass_stride, _dev(workspace), workspace_bytes)
+        n, rows = self._lens, heads << 33 | self._dim << 2 | 3
+        if q.shape != rows or out.shape != rows:
+            self._check_rows("attend", (q, out), rows)
+        rc = self._attend(self.ctx.h, self._kv, _ints(lens, n, "attend: lens"), _ints(q_off, n + 4, "attend: q_off"),
+                          max_new, heads, q, scale, out,
+                          _masses(mass_in, self._seqs, self._heads, mass_stride, "attend: mass_in"),
+                          _masses(mass_out, self._seqs, self._heads, mass_stride, "attend: mass_out"), mass_stride,
+                          _dense(workspace, workspace_bytes, "attend: workspace"), workspace_bytes)
         if rc:
             self.ctx.check(rc)
 
@@ -870,8 +948,11 @@ class Kv8Cache:
               mass_out=None, mass_out_stride: int = 0):
         """Cut every sequence to `budget` slots by accumulated mass, its kept rows written to dst's pages
         (lastro_kv8_evict)."""
-        rc = self._evict(self.ctx.h, self._kv, dst._kv, _dev(lens), budget, recent, _dev(mass), mass_stride, _dev(kept),
-                         _dev(lens_out), _dev(mass_out), mass_out_stride)
+        n, seqs, heads = self._lens, self._seqs, self._heads
+        rc = self._evict(self.ctx.h, self._kv, dst._kv, _ints(lens, n, "evict: lens"), budget, recent,
+                         _masses(mass, seqs, heads, mass_stride, "evict: mass"), mass_stride,
+                         _ints(kept, 4 * seqs * heads * budget, "evict: kept"), _ints(lens_out, n, "evict: lens_out"),
+                         _masses(mass_out, seqs, heads, mass_out_stride, "evict: mass_out"), mass_out_stride)
         if rc:
             self.ctx.check(rc)
 
@@ -879,6 +960,8 @@ class Kv8Cache:
         """The values of slots [pos0[b], pos0[b] + n) of every sequence as bf16 or f32 (lastro_kv8_read)."""
         if dtype not in ("bf16", "f32"):
             raise LastroError(E_ARG, f"dtype {dtype!r} (bf16 or f32)")
-        rc = self._read(self.ctx.h, self._kv, _dev(lens), _dev(pos0), n, _dev(k_out), _dev(v_out), _ROW_DTYPES[dtype])
+        size, kind = (n * self._slot, _BF16) if dtype == "bf16" else (2 * n * self._slot, _FLOAT32)
+        rc = self._read(self.ctx.h, self._kv, _ints(lens, self._lens, "read: lens"), _ints(pos0, self._lens, "read: pos0"), n,
+                        _dense(k_out, size, "read: k_out", kind), _dense(v_out, size, "read: v_out", kind), _ROW_DTYPES[dtype])
         if rc:
             self.ctx.check(rc)

@@ -109,3 +109,59 @@ def test_a_chain_of_calls_passes_its_results_on_the_device(ctx, fmt, dtype, new)
                 for w, x in (("k", k), ("v", v)):
                     assert np.array_equal(f64(x[b, :len(keep), h]), ref.side[b][h][w].values())
     assert src.status.item() == 0 and dst.status.item() == 0
+
+
+# ---- tensors that do not fit a call -----------------------------------------------------------------------------------------
+def test_tensors_that_do_not_fit_are_refused(ctx):
+    """of another type, place, layout or size than the call will read or write"""
+    n, kv, d, heads, room = 3, 2, 64, 4, 40
+    gpu, ref, rng = filled(ctx, "e4m3", kv, d, [20, 30, 5])
+    q, k = rows(rng, n, heads, d, "bf16"), rows(rng, n, kv, d, "bf16")
+    out, lens, off, lo = torch.zeros_like(q), ints([20, 30, 5]), ints([0, 1, 2, 3]), ints([0, 0, 0])
+    mass, kept = torch.zeros(n, kv, room, device="cuda"), torch.zeros(n, kv, 16, dtype=torch.int32, device="cuda")
+    size = gpu.c.attend_workspace(heads, 1, True)
+    work = torch.zeros(size, dtype=torch.uint8, device="cuda")
+    kr, vr = (torch.zeros(n, 8, kv, d, device="cuda") for _ in "kv")
+    ro = LB.rows_of
+    bad_ints = [lens.long(), lens.float(), lens.cpu(), lens[:2], ints([20, 0, 30, 0, 5, 0])[::2]]
+    bad_mass = [mass.double(), mass.half(), mass.cpu(), mass[:2], mass[:, :1], mass[:, :, :39].contiguous(), mass.transpose(0, 1),
+                torch.zeros(n, kv, 2 * room, device="cuda")[:, :, ::2], mass.flatten()[:-1]]
+    good_mass = [mass, mass.flatten(), torch.zeros(n, kv, room, device="cuda")[:, :, :33]]
+
+    def rows_like(x):
+        return [ro(x[:, :1]), ro(x[:, :, :32].contiguous()), ro(torch.cat([x, x], 2)), ro(torch.cat([x, x], 1)), ro(x.cpu())]
+
+    att = dict(lens=lens, q_off=off, max_new=1, heads=heads, q=ro(q), scale=0.125, out=ro(out), workspace=work, workspace_bytes=size,
+               mass_in=mass, mass_out=mass, mass_stride=room)
+    app = dict(lens=lens, new_off=off, max_new=1, k=ro(k), v=ro(k), lens_out=lo, mass=mass, mass_stride=room)
+    dst = Gpu(ctx, "e4m3", n, kv, d, 1)
+    evi = dict(dst=dst.c, lens=lens, budget=16, recent=4, mass=mass, mass_stride=room, kept=kept, lens_out=lo,
+               mass_out=torch.zeros(n, kv, 16, device="cuda"), mass_out_stride=16)
+    rd = dict(lens=lens, pos0=lo, n=8, k_out=kr, v_out=vr, dtype="f32")
+    many = [kept.long(), kept[:, :, :15].contiguous(), kept.cpu(), kept.transpose(0, 1)]
+    outs = [kr.bfloat16(), kr[:, :7].contiguous(), kr.cpu(), kr.transpose(1, 2)]
+    for f, good, bad in (
+            (gpu.c.attend, att, dict(lens=bad_ints, q_off=bad_ints + [off[:3]], q=rows_like(q), out=rows_like(out), mass_in=bad_mass,
+                                     mass_out=bad_mass, workspace=[work[:-1], work.cpu(), work.view(-1, 1)[::2]])),
+            (gpu.c.append, app, dict(lens=bad_ints, new_off=bad_ints + [off[:3]], lens_out=bad_ints, k=rows_like(k), v=rows_like(k),
+                                     mass=bad_mass)),
+            (gpu.c.evict, evi, dict(lens=bad_ints, kept=many, lens_out=bad_ints, mass=bad_mass, mass_out=[mass[:, :, :15].contiguous()])),
+            (gpu.c.read, rd, dict(lens=bad_ints, pos0=bad_ints, k_out=outs, v_out=outs))):
+        for name, values in bad.items():
+            for x in values:
+                assert code_of(f, **(good | {name: x})) == LB.E_ARG, (name, x)
+    for x in good_mass:
+        gpu.c.attend(**(att | dict(mass_in=x, mass_out=x)))
+        gpu.c.append(**(app | dict(mass=x, max_new=0, new_off=ints([0] * 4))))
+        gpu.c.evict(**(evi | dict(mass=x)))
+    gpu.c.read(**rd)
+    buffers = dict(k=gpu.k, v=gpu.v, k_scale=gpu.ks, v_scale=gpu.vs, page_table=gpu.table, status=gpu.status)
+    make = lambda b: LB.Kv8Cache(ctx, "e4m3", n, kv, d, gpu.num_pages, gpu.table.shape[1], **b)  # noqa: E731
+    make(buffers)
+    for name, t in buffers.items():
+        for x in (t.cpu(), t.flatten()[:-1], t.double()) + ((t.transpose(0, 1),) if t.ndim > 1 and name != "page_table" else ()):
+            if name in "kv" and x.dtype == torch.float64:
+                continue  # codes may be of any type, they are bytes
+            assert code_of(make, buffers | {name: x}) == LB.E_ARG, name
+    torch.cuda.synchronize()
+    assert gpu.status.item() == 0
