@@ -178,6 +178,8 @@ LDEV float key_mass(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0
 
 constexpr int kSelSlots = 16384;  // slots whose keys a CTA keeps in shared memory, after its histograms
 constexpr int kSelBins = 4096;
+// shared memory of a selection by clusters of `cl` CTAs, each with `keys` keys: the most where they are not given
+constexpr size_t sel_smem(int cl, size_t keys = kSelSlots) { return (keys + (cl > 1 ? 3 : 1) * kSelBins) * sizeof(uint32_t); }
 
 LDEV void cluster_sync() {
     asm volatile("barrier.cluster.arrive.aligned;\nbarrier.cluster.wait.aligned;" ::: "memory");
@@ -509,8 +511,8 @@ struct AppendLaunch {
     template <int FMT, int D>
     cudaError_t run() {
         const dim3 grid(blocks_of((int64_t)a.blocks * a.kv.kv_heads, 8), a.kv.n_seqs);
-        if (a.k.dtype == LASTRO_DTYPE_F32) return kv8_launch<kv8_append_kernel<FMT, D, true>>(grid, 256, 0, 1, s, a);
-        return kv8_launch<kv8_append_kernel<FMT, D, false>>(grid, 256, 0, 1, s, a);
+        if (a.k.dtype == LASTRO_DTYPE_F32) return kv8_launch<kv8_append_kernel<FMT, D, true>, 0>(grid, 256, 0, 1, s, a);
+        return kv8_launch<kv8_append_kernel<FMT, D, false>, 0>(grid, 256, 0, 1, s, a);
     }
 };
 
@@ -520,8 +522,8 @@ struct ReadLaunch {
     template <int FMT, int D>
     cudaError_t run() {
         const dim3 grid(blocks_of(a.n, 8 * kReadSlots), a.kv.n_seqs);
-        if (a.f32) return kv8_launch<kv8_read_kernel<FMT, D, true>>(grid, 256, 0, 1, s, a);
-        return kv8_launch<kv8_read_kernel<FMT, D, false>>(grid, 256, 0, 1, s, a);
+        if (a.f32) return kv8_launch<kv8_read_kernel<FMT, D, true>, 0>(grid, 256, 0, 1, s, a);
+        return kv8_launch<kv8_read_kernel<FMT, D, false>, 0>(grid, 256, 0, 1, s, a);
     }
 };
 
@@ -533,13 +535,14 @@ struct EvictLaunch {
         // a cluster where one CTA's shared memory might not hold the keys
         const int64_t slots = (int64_t)a.src.max_pages * kKv8Page;
         const int cl = slots > kSelSlots ? 8 : 1;
-        const size_t smem = ((size_t)min(((slots + cl - 1) / cl + 3) & ~(int64_t)3, (int64_t)kSelSlots) + (cl > 1 ? 3 : 1) * kSelBins) * sizeof(uint32_t);
+        const size_t keys = (size_t)min(((slots + cl - 1) / cl + 3) & ~(int64_t)3, (int64_t)kSelSlots);
+        const size_t smem = sel_smem(cl, keys);
         const dim3 grid(cl, a.src.kv_heads, a.src.n_seqs);
-        const cudaError_t e = cl > 1 ? kv8_launch<kv8_select_kernel<8>>(grid, 1024, smem, 8, s, a)
-                                     : kv8_launch<kv8_select_kernel<1>>(grid, 512, smem, 1, s, a);
+        const cudaError_t e = cl > 1 ? kv8_launch<kv8_select_kernel<8>, sel_smem(8)>(grid, 1024, smem, 8, s, a)
+                                     : kv8_launch<kv8_select_kernel<1>, sel_smem(1)>(grid, 512, smem, 1, s, a);
         if (e != cudaSuccess) return e;
         const dim3 blocks(blocks_of(a.budget, 8 * 32), a.src.kv_heads, a.src.n_seqs);
-        return kv8_launch<kv8_gather_kernel<FMT, D>>(blocks, 256, 0, 1, s, a);
+        return kv8_launch<kv8_gather_kernel<FMT, D>, 0>(blocks, 256, 0, 1, s, a);
     }
 };
 

@@ -156,18 +156,20 @@ LDEV int query_of(int r, int group) { return r < group ? 0 : r / group; }
 LDEV uint32_t warp_umax(uint32_t v) { return __reduce_max_sync(0xffffffffu, v); }
 
 // programmatic launch: the kernel's CTAs are placed while the stream's previous kernel drains and wait for its end before
-// they touch memory.  The shared memory limit of a kernel is raised once on each device.
-template <auto KERNEL, typename A>
+// they touch memory.  A kernel's shared memory limit is raised once on each device, to the most any launch of it takes, so
+// that threads which launch it at the same time set the same.
+template <auto KERNEL, size_t MOST, typename A>
 cudaError_t kv8_launch(dim3 grid, int threads, size_t smem, int cluster, cudaStream_t s, const A& a) {
-    if (smem > 48 * 1024) {
-        static std::atomic<size_t> limit[64];
+    static_assert(MOST <= 227 * 1024, "beyond what a CTA can have");
+    if (MOST > 48 * 1024) {
+        static std::atomic<bool> raised[64];
         int dev = 0;
         cudaError_t e = cudaGetDevice(&dev);
         if (e != cudaSuccess) return e;
-        if (dev >= 64 || limit[dev].load(std::memory_order_relaxed) < smem) {
-            e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (dev >= 64 || !raised[dev].load(std::memory_order_acquire)) {
+            e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)MOST);
             if (e != cudaSuccess) return e;
-            if (dev < 64) limit[dev].store(smem, std::memory_order_relaxed);
+            if (dev < 64) raised[dev].store(true, std::memory_order_release);
         }
     }
     cudaLaunchConfig_t cfg = {};

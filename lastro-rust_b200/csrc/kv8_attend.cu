@@ -1202,19 +1202,19 @@ struct AttendLaunch {
     cudaError_t go() {
         using SH = Shape<D, FEW, RW>;
         a.shares = sm_count() * (RW == 1 ? 1 : SH::GROUPS);
-        cudaError_t e = kv8_launch<kv8_attend_kernel<FMT, D, FEW, RW, F32>>(dim3(sm_count()), SH::THREADS, SH::SMEM, 1, s, a);
+        cudaError_t e = kv8_launch<kv8_attend_kernel<FMT, D, FEW, RW, F32>, SH::SMEM>(dim3(sm_count()), SH::THREADS, SH::SMEM, 1, s, a);
         if (e != cudaSuccess) return e;
         if (a.scores) {
             const dim3 blocks(min(64, (a.kv.max_pages * kKv8Page + 511) / 512), a.kv.kv_heads, a.kv.n_seqs);
-            return kv8_launch<kv8_weights_kernel<D, F32>>(blocks, 128, 0, 1, s, a);
+            return kv8_launch<kv8_weights_kernel<D, F32>, 0>(blocks, 128, 0, 1, s, a);
         }
         const int64_t rows = (int64_t)a.max_new * a.heads;
         const dim3 grid((unsigned)max((int64_t)1, min((int64_t)1024, (rows + kWarps - 1) / kWarps)), a.kv.n_seqs);
-        e = kv8_launch<kv8_merge_kernel<D, FEW, RW, F32>>(grid, kThreads, 0, 1, s, a);
+        e = kv8_launch<kv8_merge_kernel<D, FEW, RW, F32>, 0>(grid, kThreads, 0, 1, s, a);
         if (e != cudaSuccess || !a.mass_out) return e;
         const int units = a.kv.kv_heads * a.kv.n_seqs, most = (a.kv.max_pages * (kKv8Page * D / kMassChunk) + kWarps - 1) / kWarps;
         const dim3 parts(max(1, min((2 * sm_count() + units - 1) / units, most)), a.kv.kv_heads, a.kv.n_seqs);
-        return kv8_launch<kv8_mass_kernel<FMT, D, F32>>(parts, kThreads, mass_smem<D, F32>(), 1, s, a);
+        return kv8_launch<kv8_mass_kernel<FMT, D, F32>, mass_smem<D, F32>()>(parts, kThreads, mass_smem<D, F32>(), 1, s, a);
     }
     template <int FMT, int D, bool FEW, int RW>
     cudaError_t by_type() {

@@ -165,3 +165,69 @@ def test_tensors_that_do_not_fit_are_refused(ctx):
             assert code_of(make, buffers | {name: x}) == LB.E_ARG, name
     torch.cuda.synchronize()
     assert gpu.status.item() == 0
+
+
+# ---- threads --------------------------------------------------------------------------------------------------------------
+THREADS = """
+import sys, threading
+sys.path[:0] = %r
+import torch
+import lastro_b200 as LB
+
+SIZES = [256, 135, 250, 140, 2048, 258, 1500, 300] * 3  # pages: what the selection's launches take, of either kind
+sys.setswitchinterval(1e-6)
+torch.zeros(1, device="cuda")
+
+
+class Evict:
+    def __init__(self, pages):
+        self.ctx = LB.Context(0)
+        g = dict(device="cuda")
+        n, self.n = 2 * pages, pages * 64
+        self.k, self.v = torch.zeros((2, n, 1, 64, 64), dtype=torch.uint8, **g).unbind()
+        self.s = torch.ones((n, 1, 4), **g)
+        self.table = torch.arange(n, dtype=torch.int32, **g).view(2, 1, pages)
+        self.src, self.dst = (LB.Kv8Cache(self.ctx, "int8", 1, 1, 64, n, pages, self.k, self.v, self.s, self.s.clone(), t) for t in self.table)
+        self.mass = torch.arange(self.n, device="cuda").float().view(1, 1, -1)
+        self.lens, self.out = (torch.tensor([x], dtype=torch.int32, **g) for x in (self.n, 0))
+        self.kept = torch.zeros((1, 1, 100), dtype=torch.int32, **g)
+
+    def __call__(self):
+        self.src.evict(self.dst, self.lens, 100, 10, self.mass, self.n, self.kept, self.out)
+
+
+calls = [Evict(p) for p in SIZES]
+torch.cuda.synchronize()
+together, errors = threading.Barrier(len(calls)), []
+
+
+def first(c):
+    together.wait()
+    try:
+        c()
+    except LB.LastroError as e:
+        errors.append(str(e))
+
+
+threads = [threading.Thread(target=first, args=(c,)) for c in calls]
+[t.start() for t in threads]
+[t.join() for t in threads]
+for c in calls + calls[::-1]:
+    first.__globals__["together"] = threading.Barrier(1)
+    first(c)
+torch.cuda.synchronize()
+for c in calls:
+    if c.out.item() != 100 or c.kept[0, 0].tolist() != list(range(c.n - 100, c.n)):
+        errors.append("kept %%s" %% c.kept[0, 0, :4].tolist())
+sys.exit("; ".join(errors) or 0)
+"""
+
+
+def test_first_calls_from_several_threads(ctx):
+    """each with a context and a cache of another size: a launch's shared memory must not be what another thread asked for"""
+    import os
+    import subprocess
+    import sys
+    for _ in range(2):
+        r = subprocess.run([sys.executable, "-c", THREADS % [os.path.dirname(os.path.dirname(LB.__file__))]], capture_output=True, text=True)
+        assert r.returncode == 0, r.stderr[-2000:]
