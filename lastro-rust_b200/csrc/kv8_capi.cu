@@ -144,6 +144,12 @@ extern "C" int lastro_kv8_attend(lastro_ctx* ctx, const lastro_kv8* kv, const in
     a.mass_out = mass_out;
     a.mass_stride = mass_stride;
     kv8_attend_workspace(*kv, heads, max_new, mass_out != nullptr, &a, workspace);
+    if (q->rows > 0 && out->ptr == q->ptr) {  // a unit's rows are read before its outputs are written, but only by the first pass
+        if ((q->rows > 1 && q->row_stride != out->row_stride) || (heads > 1 && q->head_stride != out->head_stride))
+            return set_err(ctx, LASTRO_E_ARG, "kv8_attend: out at q's address in another layout");
+        if (mass_out && !a.scores)
+            return set_err(ctx, LASTRO_E_ARG, "kv8_attend: out must not be q, which is read again for the weights");
+    }
     if (q->rows == 0 && !mass_out) return LASTRO_OK;
     if ((int64_t)max_new * a.heads > INT32_MAX || kv8_attend_items(*kv, heads, max_new) >= (1 << 30))  // counted in 32 bits
         return set_err(ctx, LASTRO_E_UNSUPPORTED, "kv8_attend: n_seqs %d, max_pages %d, max_new %d, heads %d in one call",

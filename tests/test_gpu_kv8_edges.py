@@ -231,3 +231,28 @@ def test_first_calls_from_several_threads(ctx):
     for _ in range(2):
         r = subprocess.run([sys.executable, "-c", THREADS % [os.path.dirname(os.path.dirname(LB.__file__))]], capture_output=True, text=True)
         assert r.returncode == 0, r.stderr[-2000:]
+
+
+# ---- outputs in the queries' place ------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_outputs_over_the_queries(ctx, dtype):
+    """out may be q itself unless q is read again for the weights, which is refused, as is q's address in another layout"""
+    lens, kv, d = [300, 65, 9001], 2, 64
+    gpu, _, rng = filled(ctx, "e4m3", kv, d, lens)
+    for group, new, mass in ((3, 1, True), (3, 1, False), (2, 3, True), (2, 20, False), (1, 12, False), (3, 4, True), (1, 40, True)):
+        q, heads = [rows(rng, new, kv * group, d, dtype) for _ in lens], kv * group
+        want = gpu.attend(lens, q, 0.125, mass=mass)
+        both = torch.cat(q)
+        m = torch.full_like(want[1], -5.0) if mass else None
+        work = torch.zeros(gpu.c.attend_workspace(heads, new, mass), dtype=torch.uint8, device="cuda")
+        call = dict(lens=ints(lens), q_off=ints([0, new, 2 * new, 3 * new]), max_new=new, heads=heads, q=LB.rows_of(both), scale=0.125,
+                    out=LB.rows_of(both), workspace=work, workspace_bytes=work.numel(), mass_out=m, mass_stride=max(lens) if mass else 0)
+        if mass and group * new > 8:
+            assert code_of(gpu.c.attend, **call) == LB.E_ARG
+            continue
+        gpu.c.attend(**call)
+        assert torch.equal(both, want[0]) and (not mass or torch.equal(m, want[1]))
+    turned = torch.cat(q).transpose(0, 1).contiguous().transpose(0, 1)
+    call |= dict(q=LB.rows_of(turned), out=LB.rows_of(torch.empty(0, device="cuda").to(turned.dtype).set_(turned.untyped_storage(), 0, turned.shape)),
+                 mass_out=None, mass_stride=0)
+    assert code_of(gpu.c.attend, **call) == LB.E_ARG
