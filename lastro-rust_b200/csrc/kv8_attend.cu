@@ -19,6 +19,7 @@ namespace {
 
 constexpr int kWarps = 8, kThreads = kWarps * 32;  // of the merge and mass kernels
 constexpr float kFar = -1e30f;                    // below every score: the running maxima's start
+constexpr float kLow = -112.0f;                   // the least R - M (WarpRows): 2^(R - M - 14), which outputs are scaled by, is 2^-126
 
 LDEV float ex2(float x) {
     float y;
@@ -306,7 +307,8 @@ LDEV void score_sum(float (&s)[4], Mma mma) {
 // The running state of a row: M the ceiling of the largest score so far (scores and M in powers of two), l the sum of
 // 2^(score - M), R the ceiling of the largest score plus its slot's V exponent, o the sum of 2^(score + 14 - R) v.  M
 // and R are whole numbers, so bringing sums to new ones is exact, and R keeps the f16 weights in range whatever the
-// blocks' scales: the heaviest contribution sits between 2^13 and 2^14.  A lane holds two rows, row_of(0) and row_of(1).
+// blocks' scales: the heaviest contribution sits between 2^13 and 2^14, or lower where V's scales are below 2^-112, so that
+// the factors between them and the outputs stay in f32's range.  A lane holds two rows, row_of(0) and row_of(1).
 template <int FMT, int D, bool FEW, bool F32>
 struct WarpRows {
     static constexpr int KS = D / 16, E = FEW ? 1 : 2;
@@ -444,7 +446,7 @@ struct WarpRows {
             }
             const auto larger = [](float x, float y) { return fmaxf(x, y); };
             Mn[e] = fmaxf(M[e], ceilf(over_row(m, larger)));
-            Rn[e] = fmaxf(R[e], ceilf(over_row(r, larger)));
+            Rn[e] = fmaxf(fmaxf(R[e], ceilf(over_row(r, larger))), Mn[e] + kLow);
             moved |= Mn[e] != M[e] || Rn[e] != R[e];
         }
         if (__any_sync(0xffffffffu, moved)) {

@@ -10,7 +10,7 @@ import lastro_b200 as LB
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
-from test_gpu_kv8 import Gpu, bounds, check_attend, ctx, f64, filled, ints, rows, same_values  # noqa: E402, F401
+from test_gpu_kv8 import DT, Gpu, bounds, check_attend, ctx, f64, filled, ints, rows, same_values  # noqa: E402, F401
 
 
 def code_of(f, *a, **kw):
@@ -256,3 +256,31 @@ def test_outputs_over_the_queries(ctx, dtype):
     call |= dict(q=LB.rows_of(turned), out=LB.rows_of(torch.empty(0, device="cuda").to(turned.dtype).set_(turned.untyped_storage(), 0, turned.shape)),
                  mass_out=None, mass_stride=0)
     assert code_of(gpu.c.attend, **call) == LB.E_ARG
+
+
+# ---- values and scores far from one -----------------------------------------------------------------------------------------
+@pytest.mark.parametrize("fmt,dtype,group,new", [("e4m3", "f32", 3, 1), ("int8", "bf16", 3, 1), ("int8", "f32", 9, 1), ("e4m3", "bf16", 4, 9),
+                                                 ("e4m3", "f32", 2, 17)])
+@pytest.mark.parametrize("size", [1e-30, 1e-33, 3e-36, 1e-37])
+def test_small_values_throughout(ctx, fmt, dtype, group, new, size):
+    """V near the smallest normal f32: the outputs are as large, and as exact, as for values near one.  Beside the usual terms
+    the weights' second f16 terms lose what is below 2^-24 of the heaviest weight, for each slot, and outputs are multiples
+    of 2^-149."""
+    lens, kv, d = [500, 1, 70], 2, 64
+    rng = np.random.default_rng(31)
+    gpu, ref = Gpu(ctx, fmt, 3, kv, d, 9), R.Cache(3, kv, d, fmt)
+    k, v = [rows(rng, n, kv, d, dtype) for n in lens], [rows(rng, n, kv, d, "f32", size).to(DT[dtype]) for n in lens]
+    gpu.append([0] * 3, k, v)
+    for b in range(3):
+        ref.append(b, f64(k[b]), f64(v[b]))
+    same_values(gpu, ref, lens)
+    q, at = [rows(rng, min(new, n), kv * group, d, dtype) for n in lens], 0
+    out = f64(gpu.attend(lens, q, 0.125)[0])
+    for b, n in enumerate(lens):
+        want, _, big = ref.attend(b, f64(q[b]), 0.125)
+        vmax = max(np.abs(ref.side[b][h]["v"].values()).max() for h in range(kv))
+        _, tol = bounds(dtype, d, big, vmax)
+        tol += n * 2.0 ** -24 * vmax + 2.0 ** -149
+        got = out[at:at + len(q[b])]
+        assert (np.abs(got - want) <= tol + (2.0 ** -8 * np.abs(want) if dtype == "bf16" else 0.0)).all(), (b, np.abs(got - want).max(), tol)
+        at += len(q[b])
