@@ -18,8 +18,8 @@ namespace lastro {
 namespace {
 
 constexpr int kWarps = 8, kThreads = kWarps * 32;  // of the merge and mass kernels
-constexpr float kFar = -1e30f;                    // below every score: the running maxima's start
-constexpr float kLow = -112.0f;                   // the least R - M (WarpRows): 2^(R - M - 14), which outputs are scaled by, is 2^-126
+constexpr float kFar = -3.402823466e38f;          // no score is below it: the running maxima's start
+constexpr float kLow = -112.0f;                   // the least R (WarpRows): 2^(R - 14), which outputs are scaled by, is 2^-126
 
 LDEV float ex2(float x) {
     float y;
@@ -46,6 +46,10 @@ LDEV uint32_t transpose8(uint32_t x) {
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
+
+// A score this far from zero is a product whose rounding counts in 2^(score - M), and adding an exponent to it may round that
+// away.  M is the ceiling of rounded products; closer to zero they need not be rounded before M is taken from them.
+LDEV bool far_off(float M) { return fabsf(M) > 4096.0f && M != kFar; }
 
 // the smaller, NaN if either is
 LDEV float min_nan(float a, float b) {
@@ -305,10 +309,12 @@ LDEV void score_sum(float (&s)[4], Mma mma) {
 
 // ---- a warp's rows --------------------------------------------------------------------------------------------------------
 // The running state of a row: M the ceiling of the largest score so far (scores and M in powers of two), l the sum of
-// 2^(score - M), R the ceiling of the largest score plus its slot's V exponent, o the sum of 2^(score + 14 - R) v.  M
-// and R are whole numbers, so bringing sums to new ones is exact, and R keeps the f16 weights in range whatever the
+// 2^(score - M), R the ceiling of the largest score - M plus its slot's V exponent, o the sum of 2^(score - M + 14 - R) v.
+// M and R are whole numbers, so bringing sums to new ones is exact, and R keeps the f16 weights in range whatever the
 // blocks' scales: the heaviest contribution sits between 2^13 and 2^14, or lower where V's scales are below 2^-112, so that
-// the factors between them and the outputs stay in f32's range.  A lane holds two rows, row_of(0) and row_of(1).
+// the factors between them and the outputs stay in f32's range.  Scores of any size are as good as scores near zero: a warp
+// one of whose rows is far_off takes the branch below for every chunk (this branch, not taken, costs 24.0 -> 24.7 us at 64
+// sequences of 1024 slots with 24 heads of 64).  A lane holds two rows, row_of(0) and row_of(1).
 template <int FMT, int D, bool FEW, bool F32>
 struct WarpRows {
     static constexpr int KS = D / 16, E = FEW ? 1 : 2;
@@ -317,6 +323,7 @@ struct WarpRows {
     QFrag<D, E, F32> q;
     float o[FEW ? D / 16 : D / 8][4], M[2], R[2], l[2], g[2], fac[2];
     int vis[2];
+    bool big;  // a row's M is far_off
 
     LDEV static int row_of(int e) {
         const int lane = threadIdx.x & 31;
@@ -343,13 +350,15 @@ struct WarpRows {
 
     LDEV void begin(const Kv8AttendArgs& a, const Seq& s, int row0, const QRaw<D, E, F32>& raw) {
         q.convert(raw, a.scale);
+        big = false;
 #pragma unroll
         for (int j = 0; j < (FEW ? D / 16 : D / 8); ++j)
 #pragma unroll
             for (int i = 0; i < 4; ++i) o[j][i] = 0.0f;
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-            M[e] = R[e] = kFar;
+            M[e] = kFar;
+            R[e] = kLow;
             l[e] = g[e] = 0.0f;
             vis[e] = visible(a, s, row0 + row_of(e));
             fac[e] = FEW ? __shfl_sync(0xffffffffu, q.factor[0], 4 * row_of(e)) : q.factor[E - 1 < e ? 0 : e];
@@ -427,37 +436,59 @@ struct WarpRows {
 #pragma unroll
                         for (int k = 0; k < NT; ++k)
                             keep[row_of(e) * NB * 16 + b * 16 + slot(k)] =
-                                hidden >> ((b * 2 + e) * NT + k) & 1 ? -INFINITY : s[b][e][k] * fk[b][e];
+                                hidden >> ((b * 2 + e) * NT + k) & 1 ? -INFINITY : __fmul_rn(s[b][e][k], fk[b][e]);
         }
+        // the largest score of block b and row e
+        const auto block_top = [&](int b, int e) {
+            float top = s[b][e][0];
+#pragma unroll
+            for (int k = 1; k < NT; ++k) top = fmaxf(top, s[b][e][k]);
+            // a block that was never written has any scale, a negative one among them
+            return !WHOLE && top == -INFINITY ? top : top * fk[b][e];
+        };
+        const auto larger = [](float x, float y) { return fmaxf(x, y); };
+        const auto exponent = [](float x) { return (float)((int)(__float_as_uint(x) >> 23) - 127); };
         float Mn[2], Rn[2];
-        bool moved = false;
+        bool moved = big;
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
             float m = -INFINITY, r = -INFINITY;
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
-                float top = s[b][e][0];
-#pragma unroll
-                for (int k = 1; k < NT; ++k) top = fmaxf(top, s[b][e][k]);
-                // a block that was never written has any scale, a negative one among them
-                top = !WHOLE && top == -INFINITY ? top : top * fk[b][e];
+                const float top = block_top(b, e);
                 m = fmaxf(m, top);
-                r = fmaxf(r, top + (float)((int)(__float_as_uint(vs[b]) >> 23) - 127));
+                r = fmaxf(r, top + exponent(vs[b]));
             }
-            const auto larger = [](float x, float y) { return fmaxf(x, y); };
             Mn[e] = fmaxf(M[e], ceilf(over_row(m, larger)));
-            Rn[e] = fmaxf(fmaxf(R[e], ceilf(over_row(r, larger))), Mn[e] + kLow);
+            Rn[e] = fmaxf(fmaxf(R[e] + (M[e] - Mn[e]), ceilf(over_row(r, larger)) - Mn[e]), kLow);
             moved |= Mn[e] != M[e] || Rn[e] != R[e];
         }
         if (__any_sync(0xffffffffu, moved)) {
             float f[2];
+            big = __any_sync(0xffffffffu, far_off(Mn[0]) || far_off(Mn[1]));
+            if (big) {
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float r = -INFINITY;
+#pragma unroll
+                    for (int b = 0; b < NB; ++b) {
+#pragma unroll
+                        for (int k = 0; k < NT; ++k)
+                            if (WHOLE || !(hidden >> ((b * 2 + e) * NT + k) & 1)) s[b][e][k] = __fmul_rn(s[b][e][k], fk[b][e]);
+                        fk[b][e] = 1.0f;
+                        r = fmaxf(r, block_top(b, e) - Mn[e] + exponent(vs[b]));
+                    }
+                    Rn[e] = fmaxf(fmaxf(R[e] + (M[e] - Mn[e]), ceilf(over_row(r, larger))), kLow);
+                }
+            }
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                l[e] *= pow2i(M[e] - Mn[e]);
-                f[e] = pow2i(R[e] - Rn[e]);
+                const float up = M[e] - Mn[e];
+                l[e] *= pow2i(up);
+                f[e] = pow2i(up + (R[e] - Rn[e]));
                 M[e] = Mn[e];
                 R[e] = Rn[e];
-                g[e] = pow2i(14.0f + M[e] - R[e]);
+                g[e] = pow2i(14.0f - Rn[e]);
             }
 #pragma unroll
             for (int j = 0; j < (FEW ? D / 16 : D / 8); ++j)
@@ -577,7 +608,7 @@ struct WarpRows {
     // row e of this lane to the output: the unit is complete
     LDEV void store(const Kv8AttendArgs& a, const Seq& s, int h, int r, int e, bool vec) const {
         const int i = query_of(r, a.group), t = s.first + i, hq = h * a.group + r - i * a.group;
-        const float inv = l[e] == 0.0f ? 0.0f : 1.0f / l[e], up = pow2i(R[e] - 14.0f - M[e]);
+        const float inv = l[e] == 0.0f ? 0.0f : 1.0f / l[e], up = pow2i(R[e] - 14.0f);
 #pragma unroll
         for (int hf = 0; hf < D / 64; ++hf) {
             const int64_t at = (int64_t)t * a.out.row_stride + (int64_t)hq * a.out.head_stride + col_of(hf);
@@ -633,16 +664,17 @@ template <int D, typename At>
 LDEV void add_parts(int n, At at, float (&o)[D / 32], float& M, float& R, float& l) {
     constexpr int V = D / 32;
     const int lane = threadIdx.x & 31;
-    float4 m = make_float4(kFar, kFar, 0.0f, 0.0f);
+    float4 m = make_float4(kFar, kLow, 0.0f, 0.0f);
     if (lane < n) m = *reinterpret_cast<const float4*>(at(lane) + D);
-    float Mn = fmaxf(M, m.x), Rn = fmaxf(R, m.y);
+    float Mn = fmaxf(M, m.x), Rn = fmaxf(M + R, m.x + m.y);
 #pragma unroll
     for (int x = 16; x > 0; x >>= 1) {
         Mn = fmaxf(Mn, __shfl_xor_sync(0xffffffffu, Mn, x));
         Rn = fmaxf(Rn, __shfl_xor_sync(0xffffffffu, Rn, x));
     }
+    Rn = far_off(Mn) ? fmaxf(R + (M - Mn), warp_max(m.y + (m.x - Mn))) : Rn - Mn;
     l = l * pow2i(M - Mn) + warp_sum(m.z * pow2i(m.x - Mn));
-    const float old = pow2i(R - Rn), mine = pow2i(m.y - Rn);
+    const float old = pow2i((M - Mn) + (R - Rn)), mine = pow2i((m.x - Mn) + (m.y - Rn));
 #pragma unroll
     for (int e = 0; e < V; ++e) o[e] *= old;
     for (int i0 = 0; i0 < n; i0 += 4) {  // four parts' loads on their way at a time
@@ -676,7 +708,7 @@ template <int D, bool F32>
 LDEV void store_merged(const Kv8AttendArgs& a, int first, int h, int r, const float (&o)[D / 32], float M, float R, float l) {
     constexpr int V = D / 32;
     const int lane = threadIdx.x & 31, i = query_of(r, a.group), t = first + i, hq = h * a.group + r - i * a.group;
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l, up = pow2i(R - 14.0f - M);
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l, up = pow2i(R - 14.0f);
     const int64_t at = (int64_t)t * a.out.row_stride + (int64_t)hq * a.out.head_stride + lane * V;
 #pragma unroll
     for (int e = 0; e < V; ++e) {
@@ -933,7 +965,7 @@ __global__ void __launch_bounds__(Shape<D, FEW, RW>::THREADS, 1) kv8_attend_kern
         const int first = max(which, 0), nrows = min(SH::ROWS, (which < 0 ? x.hn : x.tn) * a.group - tile * TILE);
         for (int r = 0; r < nrows; ++r, ++task) {
             if (task % SH::WARPS != warp) continue;
-            float o[D / 32] = {}, M = kFar, R = kFar, l = 0.0f;
+            float o[D / 32] = {}, M = kFar, R = kLow, l = 0.0f;
             add_parts<D>(n, [&](int i) -> const float* {
                 if (which >= 0 && i == 0)
                     return reinterpret_cast<const float*>(smem + (size_t)first * ST * STAGE) + r * SH::PART;
@@ -968,7 +1000,7 @@ __global__ void __launch_bounds__(kThreads) kv8_merge_kernel(const __grid_consta
         const int i = u / a.heads, hq = u - i * a.heads, h = hq / a.group, r = i * a.group + hq - h * a.group, tile = r / SH::TILE;
         const int first = base + (h * s.tiles + tile) * s.chunks, g0 = first / per, g1 = (first + s.chunks - 1) / per;
         if (g0 == g1) continue;
-        float o[D / 32] = {}, M = kFar, R = kFar, l = 0.0f;
+        float o[D / 32] = {}, M = kFar, R = kLow, l = 0.0f;
         for (int g = g0; g <= g1; g += 32)
             add_parts<D>(min(32, g1 + 1 - g), [&](int k) {
                 return a.part + (((int64_t)(g + k) * 2 + (g + k == g0)) * SH::TILE + r - tile * SH::TILE) * SH::PART;
@@ -1000,13 +1032,13 @@ __global__ void __launch_bounds__(128) kv8_weights_kernel(const __grid_constant_
             continue;
         }
         const auto part = [&](int g) { return a.part + (((int64_t)g * 2 + (g == g0)) * SH::TILE + r) * SH::PART; };
-        float o[D / 32] = {}, M = kFar, R = kFar, l = 0.0f;
+        float o[D / 32] = {}, M = kFar, R = kLow, l = 0.0f;
         for (int g = g0; g <= g1; g += 32) {
             const int n = min(32, g1 + 1 - g);
             if (blockIdx.x == 0) {
                 add_parts<D>(n, [&](int k) { return part(g + k); }, o, M, R, l);
             } else {
-                const float4 m = lane < n ? *reinterpret_cast<const float4*>(part(g + lane) + D) : make_float4(kFar, kFar, 0.0f, 0.0f);
+                const float4 m = lane < n ? *reinterpret_cast<const float4*>(part(g + lane) + D) : make_float4(kFar, kLow, 0.0f, 0.0f);
                 const float Mn = fmaxf(M, warp_max(m.x));
                 l = l * pow2i(M - Mn) + warp_sum(m.z * pow2i(m.x - Mn));
                 M = Mn;

@@ -284,3 +284,31 @@ def test_small_values_throughout(ctx, fmt, dtype, group, new, size):
         got = out[at:at + len(q[b])]
         assert (np.abs(got - want) <= tol + (2.0 ** -8 * np.abs(want) if dtype == "bf16" else 0.0)).all(), (b, np.abs(got - want).max(), tol)
         at += len(q[b])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("group,new", [(3, 1), (9, 1), (4, 9)])
+@pytest.mark.parametrize("score", [2.0 ** 20, 2.0 ** 27, 2.0 ** 40, 1e35])
+def test_scores_far_from_zero(ctx, dtype, group, new, score):
+    """every slot has the same score, far from zero on either side: the same bits for all, so every weight is the same and an
+    output is the mean of the values it sees, whatever their scales are"""
+    lens, kv, d = [9001, 33], 1, 64
+    rng = np.random.default_rng(33)
+    k = torch.zeros(max(lens), kv, d)
+    k[:, :, 0] = score
+    for size in (1.0, 1e4, 1e-6):
+        gpu, ref = Gpu(ctx, "int8", 2, kv, d, 141), R.Cache(2, kv, d, "int8")
+        v = [rows(rng, n, kv, d, "f32", size) for n in lens]
+        gpu.append([0, 0], [k[:n].cuda() for n in lens], v)
+        for b in range(2):
+            ref.append(b, f64(k[:lens[b]]), f64(v[b]))
+        q = [rows(rng, new, group, d, dtype) for _ in lens]
+        for x in q:
+            x[:, :, 0] = torch.tensor([1.0, -1.0])[torch.arange(group) % 2].to(x)
+        out = f64(gpu.attend(lens, q, 1.0)[0])
+        for b, n in enumerate(lens):
+            x = ref.side[b][0]["v"].values()
+            for i in range(new):
+                want = x[:n - new + i + 1].mean(0)
+                tol = np.abs(x).max() * (2.0 ** -20 + (2.0 ** -11 if dtype == "bf16" else 0.0)) + (2.0 ** -8 * np.abs(want) if dtype == "bf16" else 0.0)
+                assert (np.abs(out[b * new + i] - want) <= tol).all(), (size, b, i)
