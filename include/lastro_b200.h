@@ -374,8 +374,8 @@ int lastro_kv8_attend_workspace(lastro_ctx *ctx, const lastro_kv8 *kv, int32_t h
  * finite gets NaN.  out may be q itself (the same address and strides), except, which is refused, where q is read again for
  * the weights: with mass_out and more than 8 query rows to a KV head (max_new * group) or more than 1 GiB of scores (one
  * float for each row and each slot that the page table can name); else it must not overlap q.  mass_out, when not NULL: [n_seqs, kv_heads, mass_stride] with mass_out[b, h, t] = mass_in[b, h, t] (0
- * when mass_in is NULL) + the attention weights slot t received from every query and every head of group h, for
- * t < lens[b]; other entries are not written; mass_in may be mass_out.  Products accumulate in f32; bf16 rows are exact
+ * when mass_in is NULL) + the attention weights slot t received from every query and every head of group h (NaN from one
+ * that sees it and whose output is NaN for its own values or K's), for t < lens[b]; other entries are not written; mass_in may be mass_out.  Products accumulate in f32; bf16 rows are exact
  * operands and their weights are rounded to f16 (11 bits, below the output's 8), f32 rows and weights are carried as two
  * f16 terms (22 bits).  The same call on the same data gives the same bits. */
 int lastro_kv8_attend(lastro_ctx *ctx, const lastro_kv8 *kv, const int32_t *lens, const int32_t *q_off, int32_t max_new,

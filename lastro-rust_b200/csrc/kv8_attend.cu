@@ -1062,8 +1062,9 @@ __global__ void __launch_bounds__(128) kv8_weights_kernel(const __grid_constant_
             for (int r = 0; r < 8; ++r)
                 if (r < rows) {
                     const float4 v = *reinterpret_cast<const float4*>(src + r * SH::TOK);
-                    sum[0] += ex2(v.x - lse[r]), sum[1] += ex2(v.y - lse[r]);
-                    sum[2] += ex2(v.z - lse[r]), sum[3] += ex2(v.w - lse[r]);
+                    // the row's sum may be NaN, which is for the slots it sees
+                    const auto weight = [&](float x) { return x == -INFINITY ? 0.0f : ex2(x - lse[r]); };
+                    sum[0] += weight(v.x), sum[1] += weight(v.y), sum[2] += weight(v.z), sum[3] += weight(v.w);
                 }
         }
         if (vec && t + 4 <= s.len) {

@@ -312,3 +312,26 @@ def test_scores_far_from_zero(ctx, dtype, group, new, score):
                 want = x[:n - new + i + 1].mean(0)
                 tol = np.abs(x).max() * (2.0 ** -20 + (2.0 ** -11 if dtype == "bf16" else 0.0)) + (2.0 ** -8 * np.abs(want) if dtype == "bf16" else 0.0)
                 assert (np.abs(out[b * new + i] - want) <= tol).all(), (size, b, i)
+
+
+# ---- weights ------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("group,new", [(2, 3), (1, 8), (3, 7), (2, 40)])
+def test_weights_of_rows_that_are_not_finite_stay_apart(ctx, dtype, group, new):
+    """a query that holds NaN or infinity gives NaN to the slots it sees and nothing to the others; what a page outside the
+    pool would hold gets nothing"""
+    lens, kv, d = [100, 50], 1, 64
+    gpu, _, rng = filled(ctx, "e4m3", kv, d, lens)
+    q = [rows(rng, new, group, d, dtype) for _ in lens]
+    _, clean = gpu.attend(lens, q, 0.125, mass=True)
+    for bad in (math.nan, math.inf):
+        x = [t.clone() for t in q]
+        x[0][1, 0, 5] = bad
+        _, mass = gpu.attend(lens, x, 0.125, mass=True)
+        see = lens[0] - new + 2  # slots that query 1 sees
+        assert mass[0, :, :see].isnan().all() and torch.equal(mass[0, :, see:], clean[0, :, see:])
+        assert torch.equal(mass[1], clean[1])
+    assert gpu.status.item() == 0
+    gpu.table[0, 0] = -1
+    _, mass = gpu.attend(lens, x, 0.125, mass=True)
+    assert (mass[0, :, :64] == 0).all() and torch.equal(mass[1], clean[1]) and gpu.status.item() == LB.KV8_BAD_PAGE
