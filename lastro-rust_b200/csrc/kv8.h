@@ -33,7 +33,9 @@ struct Kv8AttendArgs {
     // workspace (kv8_attend_workspace)
     int32_t* offset;       // [n_seqs + 1]: where each sequence's work starts in the list, the list's length
     float* part;           // partial results of units cut between shares of the list
-    float* lse;            // [rows, heads]: log2 of each softmax's sum, what the weights are rebuilt from; NULL without them
+    // [rows, heads]: each softmax's maximum (in powers of two) and 1 / sum, which the weights are rebuilt from; NULL without
+    // them.  Not the logarithm of both, which far from zero would round the sum away.
+    float2* norm;
     float* scores;         // [list items][score_rows][chunk's slots]: the scores, where they are kept
     int32_t shares, score_rows;
 };

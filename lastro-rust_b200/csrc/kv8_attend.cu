@@ -640,7 +640,7 @@ struct WarpRows {
                 }
             }
         }
-        if (a.lse && first_of_row()) a.lse[(int64_t)t * a.heads + hq] = l[e] == 0.0f ? INFINITY : M[e] + log2f(l[e]);
+        if (a.norm && first_of_row()) a.norm[(int64_t)t * a.heads + hq] = make_float2(M[e], inv);
     }
 
     // row e of this lane as a partial result
@@ -718,7 +718,7 @@ LDEV void store_merged(const Kv8AttendArgs& a, int first, int h, int r, const fl
         else
             static_cast<uint16_t*>(a.out.ptr)[at + e] = f32_to_bf16_rne(v);
     }
-    if (a.lse && lane == 0) a.lse[(int64_t)t * a.heads + hq] = l == 0.0f ? INFINITY : M + log2f(l);
+    if (a.norm && lane == 0) a.norm[(int64_t)t * a.heads + hq] = make_float2(M, inv);
 }
 
 // ---- one pass over the cache ----------------------------------------------------------------------------------------------
@@ -1017,7 +1017,7 @@ __global__ void __launch_bounds__(kThreads) kv8_merge_kernel(const __grid_consta
 template <int D, bool F32>
 __global__ void __launch_bounds__(128) kv8_weights_kernel(const __grid_constant__ Kv8AttendArgs a) {
     using SH = Shape<D, true, 1>;
-    __shared__ float sums[SH::ROWS];
+    __shared__ float2 norms[SH::ROWS];
     pdl_wait();
     pdl_launch();
     const int b = blockIdx.z, h = blockIdx.y, H = a.kv.kv_heads, lane = threadIdx.x & 31;
@@ -1028,7 +1028,7 @@ __global__ void __launch_bounds__(128) kv8_weights_kernel(const __grid_constant_
     for (int r = threadIdx.x >> 5; r < rows; r += 4) {
         if (g0 == g1) {
             const int i = query_of(r, a.group);
-            if (lane == 0) sums[r] = a.lse[(int64_t)(s.first + i) * a.heads + h * a.group + r - i * a.group];
+            if (lane == 0) norms[r] = a.norm[(int64_t)(s.first + i) * a.heads + h * a.group + r - i * a.group];
             continue;
         }
         const auto part = [&](int g) { return a.part + (((int64_t)g * 2 + (g == g0)) * SH::TILE + r) * SH::PART; };
@@ -1045,13 +1045,13 @@ __global__ void __launch_bounds__(128) kv8_weights_kernel(const __grid_constant_
             }
         }
         if (blockIdx.x == 0) store_merged<D, F32>(a, s.first, h, r, o, M, R, l);
-        if (lane == 0) sums[r] = l == 0.0f ? INFINITY : M + log2f(l);
+        if (lane == 0) norms[r] = make_float2(M, l == 0.0f ? 0.0f : 1.0f / l);
     }
     __syncthreads();
-    float lse[SH::ROWS];
+    float2 norm[SH::ROWS];
 #pragma unroll
     for (int r = 0; r < SH::ROWS; ++r)
-        if (r < rows) lse[r] = sums[r];
+        if (r < rows) norm[r] = norms[r];
     const int64_t at = ((int64_t)b * H + h) * a.mass_stride;
     const bool vec = ((reinterpret_cast<uintptr_t>(a.mass_out + at) | reinterpret_cast<uintptr_t>(a.mass_in ? a.mass_in + at : nullptr)) & 15) == 0;
     for (int t = (blockIdx.x * 128 + threadIdx.x) * 4; t < s.len; t += gridDim.x * 512) {
@@ -1063,8 +1063,10 @@ __global__ void __launch_bounds__(128) kv8_weights_kernel(const __grid_constant_
                 if (r < rows) {
                     const float4 v = *reinterpret_cast<const float4*>(src + r * SH::TOK);
                     // the row's sum may be NaN, which is for the slots it sees
-                    const auto weight = [&](float x) { return x == -INFINITY ? 0.0f : ex2(x - lse[r]); };
-                    sum[0] += weight(v.x), sum[1] += weight(v.y), sum[2] += weight(v.z), sum[3] += weight(v.w);
+                    const auto add = [&](float& to, float x) {
+                        if (x != -INFINITY) to = fmaf(ex2(x - norm[r].x), norm[r].y, to);
+                    };
+                    add(sum[0], v.x), add(sum[1], v.y), add(sum[2], v.z), add(sum[3], v.w);
                 }
         }
         if (vec && t + 4 <= s.len) {
@@ -1087,7 +1089,7 @@ constexpr int kMassTiles = kWarps, kMassChunk = 2048;  // query tiles in shared 
 
 template <int D, bool F32>
 constexpr size_t mass_smem() {
-    return (size_t)kMassTiles * (D / 16) * 32 * 16 * (F32 ? 2 : 1) + kMassTiles * 16 * 3 * 4 + kWarps * 64 * 4;
+    return (size_t)kMassTiles * (D / 16) * 32 * 16 * (F32 ? 2 : 1) + kMassTiles * 16 * 4 * 4 + kWarps * 64 * 4;
 }
 
 template <int FMT, int D, bool F32>
@@ -1097,9 +1099,9 @@ __global__ void __launch_bounds__(kThreads, 2) kv8_mass_kernel(const __grid_cons
     pdl_wait();
     pdl_launch();
     uint4* qs = reinterpret_cast<uint4*>(smem);  // [tile][ks][lane], first terms then second ones
-    float* rfac = reinterpret_cast<float*>(qs + (size_t)kMassTiles * KS * 32 * (F32 ? 2 : 1));
-    float* rlse = rfac + kMassTiles * 16;
-    int* rvis = reinterpret_cast<int*>(rlse + kMassTiles * 16);
+    float2* rnorm = reinterpret_cast<float2*>(qs + (size_t)kMassTiles * KS * 32 * (F32 ? 2 : 1));
+    float* rfac = reinterpret_cast<float*>(rnorm + kMassTiles * 16);
+    int* rvis = reinterpret_cast<int*>(rfac + kMassTiles * 16);
     float* sums = reinterpret_cast<float*>(rvis + kMassTiles * 16) + (threadIdx.x >> 5) * 64;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gq = lane >> 2, c4 = lane & 3, H = a.kv.kv_heads;
     const bool vq = vec_rows(a.q);
@@ -1145,7 +1147,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv8_mass_kernel(const __grid_cons
                     const int r = row0 + gq + 8 * e, at = warp * 16 + gq + 8 * e, i = r / a.group;
                     rfac[at] = q.factor[e];
                     rvis[at] = visible(a, s, r);
-                    rlse[at] = r < rows ? a.lse[(int64_t)(s.first + i) * a.heads + h * a.group + r - i * a.group] : INFINITY;
+                    rnorm[at] = r < rows ? a.norm[(int64_t)(s.first + i) * a.heads + h * a.group + r - i * a.group] : make_float2(0.0f, 0.0f);
                 }
         }
         __syncthreads();
@@ -1171,8 +1173,9 @@ __global__ void __launch_bounds__(kThreads, 2) kv8_mass_kernel(const __grid_cons
                         if (F32) p[F32 ? k : 0] = qs[((kMassTiles + t) * KS + k) * 32 + lane];
                     }
                     const float fac[2] = {rfac[t * 16 + gq], rfac[t * 16 + gq + 8]};
-                    const float lse[2] = {rlse[t * 16 + gq], rlse[t * 16 + gq + 8]};
+                    const float2 norm[2] = {rnorm[t * 16 + gq], rnorm[t * 16 + gq + 8]};
                     const int vis[2] = {rvis[t * 16 + gq], rvis[t * 16 + gq + 8]};
+                    const bool far = __any_sync(0xffffffffu, far_off(norm[0].x) || far_off(norm[1].x));  // as the first pass rounded
 #pragma unroll
                     for (int n = 0; n < NB; ++n)
 #pragma unroll
@@ -1184,9 +1187,10 @@ __global__ void __launch_bounds__(kThreads, 2) kv8_mass_kernel(const __grid_cons
                             });
 #pragma unroll
                             for (int i = 0; i < 4; ++i) {
-                                float v = ex2(x[i] * (fac[i >> 1] * ks[n]) - lse[i >> 1]);
-                                if (!whole && c * TOK + n * 16 + slot_of(c4, i & 1, j) >= vis[i >> 1]) v = 0.0f;
-                                sum[n][j][i & 1] += v;
+                                const float f = fac[i >> 1] * ks[n], M = norm[i >> 1].x;
+                                const float v = ex2(far ? __fmul_rn(x[i], f) - M : fmaf(x[i], f, -M));
+                                if (whole || c * TOK + n * 16 + slot_of(c4, i & 1, j) < vis[i >> 1])
+                                    sum[n][j][i & 1] = fmaf(v, norm[i >> 1].y, sum[n][j][i & 1]);
                             }
                         }
                 }
@@ -1275,7 +1279,7 @@ size_t kv8_attend_workspace(const lastro_kv8& kv, int heads, int max_new, bool w
     const size_t row = (kv.head_dim + 4) * sizeof(float), shares = (size_t)sm_count() * (rw <= 1 ? 1 : 8 / rw);
     const size_t offset = align16(((size_t)kv.n_seqs + 1) * sizeof(int32_t));
     const size_t part = shares * 2 * (rw ? rw * 16 : 8) * row;
-    const size_t lse = with_mass ? align16((size_t)kv.n_seqs * max_new * heads * sizeof(float)) : 0;
+    const size_t norm = with_mass ? align16((size_t)kv.n_seqs * max_new * heads * sizeof(float2)) : 0;
     // kept scores save the second pass over K; past 1 GiB of them K is read again instead
     size_t scores = with_mass && rw == 0 ? (size_t)kv.n_seqs * kv.kv_heads * kv.max_pages * kKv8Page * rows * sizeof(float) : 0;
     if (scores > ((size_t)1 << 30)) scores = 0;
@@ -1283,11 +1287,11 @@ size_t kv8_attend_workspace(const lastro_kv8& kv, int heads, int max_new, bool w
         unsigned char* p = static_cast<unsigned char*>(base);
         a->offset = reinterpret_cast<int32_t*>(p);
         a->part = reinterpret_cast<float*>(p + offset);
-        a->lse = with_mass ? reinterpret_cast<float*>(p + offset + part) : nullptr;
-        a->scores = scores ? reinterpret_cast<float*>(p + offset + part + lse) : nullptr;
+        a->norm = with_mass ? reinterpret_cast<float2*>(p + offset + part) : nullptr;
+        a->scores = scores ? reinterpret_cast<float*>(p + offset + part + norm) : nullptr;
         a->score_rows = (int32_t)rows;
     }
-    return offset + part + lse + scores;
+    return offset + part + norm + scores;
 }
 
 int64_t kv8_attend_items(const lastro_kv8& kv, int heads, int max_new) {

@@ -335,3 +335,20 @@ def test_weights_of_rows_that_are_not_finite_stay_apart(ctx, dtype, group, new):
     gpu.table[0, 0] = -1
     _, mass = gpu.attend(lens, x, 0.125, mass=True)
     assert (mass[0, :, :64] == 0).all() and torch.equal(mass[1], clean[1]) and gpu.status.item() == LB.KV8_BAD_PAGE
+
+
+@pytest.mark.parametrize("group,new", [(3, 1), (2, 4), (3, 7)])
+@pytest.mark.parametrize("score", [0.0, 1e5, 2.0 ** 23, 1e9, -1e5, -1e9, -1e30])
+def test_weights_of_scores_far_from_zero(ctx, group, new, score):
+    """every slot has the same score: each gets the same weight, and a row hands out 1"""
+    lens, kv, d = [5000, 40], 1, 64
+    k = torch.zeros(max(lens), kv, d, device="cuda")
+    k[:, :, 0] = score
+    gpu = Gpu(ctx, "int8", 2, kv, d, 79)
+    gpu.append([0, 0], [k[:n] for n in lens], [k[:n] for n in lens])
+    q = torch.zeros(new, group, d, device="cuda")
+    q[:, :, 0] = 1.0
+    _, mass = gpu.attend(lens, [q, q], 1.0, mass=True)
+    for b, n in enumerate(lens):
+        want = sum(group * (torch.arange(n) < n - new + i + 1).double() / (n - new + i + 1) for i in range(new))
+        assert (np.abs(f64(mass[b, 0, :n]) - want.numpy()) <= 2.0 ** -20 * want.numpy()).all()
