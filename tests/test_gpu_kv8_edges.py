@@ -352,3 +352,13 @@ def test_weights_of_scores_far_from_zero(ctx, group, new, score):
     for b, n in enumerate(lens):
         want = sum(group * (torch.arange(n) < n - new + i + 1).double() / (n - new + i + 1) for i in range(new))
         assert (np.abs(f64(mass[b, 0, :n]) - want.numpy()) <= 2.0 ** -20 * want.numpy()).all()
+
+
+# ---- prompts -------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("fmt,kv,group,d,dtype", [("e4m3", 2, 3, 64, "bf16"), ("int8", 1, 4, 128, "f32"), ("int8", 1, 1, 64, "bf16")])
+def test_attention_over_a_prompt(ctx, fmt, kv, group, d, dtype):
+    """hundreds of queries a sequence, some of them all of its slots, with and without the weights"""
+    lens, news = [700, 513, 64, 900], [700, 257, 64, 1]
+    gpu, ref, rng = filled(ctx, fmt, kv, d, lens)
+    check_attend(gpu, ref, rng, lens, news, kv * group, dtype)
+    check_attend(gpu, ref, rng, lens, news, kv * group, dtype, with_mass=False)
