@@ -151,7 +151,9 @@ extern "C" int lastro_kv8_attend(lastro_ctx* ctx, const lastro_kv8* kv, const in
             return set_err(ctx, LASTRO_E_ARG, "kv8_attend: out must not be q, which is read again for the weights");
     }
     if (q->rows == 0 && !mass_out) return LASTRO_OK;
-    if ((int64_t)max_new * a.heads > INT32_MAX || kv8_attend_items(*kv, heads, max_new) >= (1 << 30))  // counted in 32 bits
+    // counted in 32 bits, the rows that a sequence can have in steps of up to 8192
+    if ((int64_t)max_new * a.heads > INT32_MAX || (int64_t)std::min(max_new, q->rows) * a.heads > INT32_MAX - 8192 ||
+        kv8_attend_items(*kv, heads, max_new) >= (1 << 30))
         return set_err(ctx, LASTRO_E_UNSUPPORTED, "kv8_attend: n_seqs %d, max_pages %d, max_new %d, heads %d in one call",
                        kv->n_seqs, kv->max_pages, max_new, heads);
     KV8_TRY(on_device(ctx, "kv8_attend"));

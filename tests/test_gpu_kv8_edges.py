@@ -48,6 +48,20 @@ def test_append_of_more_rows_than_can_be_counted_is_refused(ctx):
     assert gpu.status.item() == 0
 
 
+def test_attention_of_more_rows_than_can_be_counted_is_refused(ctx):
+    """rows times heads right up to 2^31; the bound alone, with few rows, is taken"""
+    gpu, ref, rng = filled(ctx, "e4m3", 1, 64, [20], max_pages=1)
+    q, most = rows(rng, 3, 1, 64, "f32"), 2 ** 31 - 1
+    out = torch.zeros_like(q)
+    work = torch.zeros(gpu.c.attend_workspace(1, most, False), dtype=torch.uint8, device="cuda")
+    many = [LB.Rows(x.data_ptr(), LB.DTYPE_F32, most, 0, 0) for x in (q, out)]
+    call = dict(lens=ints([20]), q_off=ints([0, 3]), max_new=most, heads=1, scale=0.125, workspace=work, workspace_bytes=work.numel())
+    assert code_of(gpu.c.attend, **call, q=many[0], out=many[1]) == LB.E_UNSUPPORTED
+    gpu.c.attend(**call, q=LB.rows_of(q), out=LB.rows_of(out))
+    want, _, big = ref.attend(0, f64(q), 0.125)
+    assert (np.abs(f64(out) - want) <= bounds("f32", 64, big, np.abs(ref.side[0][0]["v"].values()).max())[1]).all()
+
+
 # ---- shared memory ------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("news", [1, 12])
 def test_copies_that_follow_the_list_closely(ctx, news):
