@@ -3,8 +3,8 @@
 A batch of sequences is decoded greedily by a one-layer model with random weights (embedding, q/k/v/o projections of the
 1B Granite's heads, an untied head).  Each step appends the new tokens' K and V to the cache, attends over it while the
 weights that each slot receives accumulate, and, once the longest sequence reaches `limit` slots, evicts every sequence to
-`budget` slots: the latest `recent` and the heaviest of the others.  Memory is that of `limit` slots however long the
-sequences get.
+`budget` slots: the latest `recent` and the heaviest of the others.  Memory is that of two caches of `limit` slots (eviction
+writes from one to the other) however long the sequences get.
 
     python examples/bounded_decode.py --tokens 300 --limit 256 --budget 128
 """
@@ -104,6 +104,8 @@ def main():
     ap.add_argument("--recent", type=int, default=32)
     ap.add_argument("--format", choices=sorted(LB.KV8_FORMATS), default="e4m3")
     a = ap.parse_args()
+    if not (0 <= a.recent <= a.budget < a.limit and a.budget > 0):
+        ap.error("0 <= recent <= budget, 0 < budget < limit")
     ids, cache = decode(a.sequences, a.tokens, a.limit, a.budget, a.recent, a.format)
     for b in range(a.sequences):
         print(f"sequence {b}: {ids[b, :12].tolist()} ...")

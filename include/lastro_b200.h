@@ -330,9 +330,10 @@ void lastro_batch_destroy(lastro_batch *batch);
  * a value that is not finite gets a NaN scale: all of it reads as NaN.  (Magnitudes above 3.2e38 may round to infinity.)
  * Sequence lengths and row offsets are read on the device.  What the host cannot check there is checked by the kernels:
  * a page number outside the pool, a length outside the page table, row offsets outside the rows or beyond max_new make
- * the kernel skip that page or sequence and leave a LASTRO_KV8_BAD_* code in *status (device memory, may be NULL; never
- * cleared by the library).  Slots, blocks and pages that hold no row may hold any bits; the e4m3 codes of NaN (0x7f, 0xff)
- * are never written and are not looked for in rows.  Calls that share a cache, a workspace or outputs must not overlap on the GPU. */
+ * the kernel skip that page or sequence (queries of a length that does not fit see nothing) and leave a LASTRO_KV8_BAD_*
+ * code in *status (device memory, may be NULL; never cleared by the library).  Slots, blocks and pages that hold no row
+ * may hold any bits; the e4m3 codes of NaN (0x7f, 0xff) are never written and are not looked for in rows.  Calls that
+ * share a cache, a workspace or outputs must not overlap on the GPU. */
 #define LASTRO_KV8_E4M3 1
 #define LASTRO_KV8_INT8 2
 #define LASTRO_KV8_PAGE 64
@@ -369,15 +370,18 @@ int lastro_kv8_append(lastro_ctx *ctx, const lastro_kv8 *kv, const int32_t *lens
 int lastro_kv8_attend_workspace(lastro_ctx *ctx, const lastro_kv8 *kv, int32_t heads, int32_t max_new,
                                 int32_t with_mass, size_t *bytes);
 /* grouped-query attention over the cache: rows [q_off[b], q_off[b + 1]) of q (heads a multiple of kv_heads; at most
- * n_seqs * max_new rows in all) are the last queries of sequence b, whose length lens[b] counts their own slots: query i of n sees slots [0, lens[b] - n + i].
- * out = softmax(scale * q k) v in q's dtype; a query that sees no slot gets zeros, one that holds a value that is not
- * finite gets NaN.  out may be q itself (the same address and strides), except, which is refused, where q is read again for
- * the weights: with mass_out and more than 8 query rows to a KV head (max_new * group) or more than 1 GiB of scores (one
- * float for each row and each slot that the page table can name); else it must not overlap q.  mass_out, when not NULL: [n_seqs, kv_heads, mass_stride] with mass_out[b, h, t] = mass_in[b, h, t] (0
+ * n_seqs * max_new rows in all) are the last queries of sequence b, whose length lens[b] counts their own slots: query i
+ * of n sees slots [0, lens[b] - n + i]. out = softmax(scale * q k) v in q's dtype; a query that sees no slot gets zeros,
+ * one that holds a value that is not finite gets NaN.  out may be q itself (the same address and strides), except, which
+ * is refused, where q is read again for the weights: with mass_out and more than 8 query rows to a KV head (max_new *
+ * group) or more than 1 GiB of scores (one float for each row and each slot that the page table can name); else it must
+ * not overlap q.  mass_out, when not NULL: [n_seqs, kv_heads, mass_stride] with mass_out[b, h, t] = mass_in[b, h, t] (0
  * when mass_in is NULL) + the attention weights slot t received from every query and every head of group h (NaN from one
- * that sees it and whose output is NaN for its own values or K's), for t < lens[b]; other entries are not written; mass_in may be mass_out.  Products accumulate in f32; bf16 rows are exact
- * operands and their weights are rounded to f16 (11 bits, below the output's 8), f32 rows and weights are carried as two
- * f16 terms (22 bits).  The same call on the same data gives the same bits. */
+ * that sees it and whose output is NaN for its own values or K's), for t < lens[b]; other entries are not written;
+ * mass_in may be mass_out.  Products accumulate in f32: bf16 rows are exact operands, their weights are rounded to f16
+ * (11 bits, below the output's 8) and the weighted sums stay in the matrix unit, which cuts off what is below f32 (at
+ * most a unit in the last place for each 16 slots); f32 rows and weights are carried as two f16 terms (22 bits) and
+ * their sums rounded.  Scores are f32 of any size.  The same call on the same data gives the same bits. */
 int lastro_kv8_attend(lastro_ctx *ctx, const lastro_kv8 *kv, const int32_t *lens, const int32_t *q_off, int32_t max_new,
                       int32_t heads, const lastro_rows *q, float scale, const lastro_rows *out, const float *mass_in,
                       float *mass_out, int64_t mass_stride, void *workspace, size_t workspace_bytes);

@@ -10,8 +10,9 @@ namespace {
 // ---- append ---------------------------------------------------------------------------------------------------------
 // One warp quantises one block (16 slots) of K and V of one head: its new rows are read once into registers (a lane holds
 // groups of 8 values), the largest magnitude comes by a warp reduction, then the codes.  The block's earlier rows are read
-// and rounded again only where the scale grows.  Bound by memory, 2 or 4 bytes a value in and 1 out: 44 us for 8 x 4097 rows
-// of 8 heads of 128 in bf16 (201 MB, 4.6 TB/s); one row each for 64 sequences takes 3.3 us, four dependent loads.
+// and rounded again only where the scale grows.  Bound by memory, 2 or 4 bytes a value in and 1 out, and by loads that each
+// warp has on its way only once: 41 us for 28,678 rows of 8 sequences, 8 heads of 128 in bf16 (177 MB, 4.4 TB/s); one row each
+// for 64 sequences takes 3.2 us, four dependent loads.
 template <int FMT, int D, bool F32>
 __global__ void __launch_bounds__(256) kv8_append_kernel(const __grid_constant__ Kv8AppendArgs a) {
     constexpr int LPR = D / 8, RPW = 32 / LPR, N = kKv8Block / RPW;  // lanes a row, rows a pass, passes
@@ -104,8 +105,8 @@ __global__ void __launch_bounds__(256) kv8_append_kernel(const __grid_constant__
 
 // ---- read-back ------------------------------------------------------------------------------------------------------
 // One warp takes kReadSlots slots of a sequence, all heads: a lane turns 8 codes into 16 or 32 bytes, so that a warp's stores
-// are whole lines (16 codes a lane, whose stores leave gaps for the next, ran at half the rate).  Bound by memory: 32 us for
-// 8 x 4113 slots of 8 heads of 128 (202 MB, 6.3 TB/s, some of it still in L2).
+// are whole lines (16 codes a lane, whose stores leave gaps for the next, ran at half the rate).  Bound by memory: 33 us for
+// 8 x 4113 slots of 8 heads of 128, 28,747 of them held (194 MB, 5.9 TB/s, some of it still in L2).
 constexpr int kReadSlots = 2;
 
 template <int FMT, int D, bool F32>
@@ -208,8 +209,8 @@ LDEV uint32_t ld_cluster(const uint32_t* p, uint32_t rank) {
 // 10 bits: masses share their leading bits, and 8-bit digits had most of them counted in a few words, one at a time), whose
 // counts every CTA adds to all the others' (few are not zero).  Then one pass writes the kept slots in order, all above the
 // key and of those at it the lowest: a warp takes consecutive slots and knows from counts what is kept before them.  Bound
-// by its barriers and shared memory: 19 us for 64 x 8 heads of 4097 slots (512 CTAs at once), 33 us for 2 x 8 of 131072 (16
-// clusters), 6.5 us for 8 of 2049.
+// by its barriers and shared memory: 18 us for 64 x 8 heads of 3097 to 4097 slots (512 CTAs at once), 32 us for 2 x 8 of
+// 123,153 and 131,072 (16 clusters), 6.4 us for 8 of 2049.
 template <int CL>
 __global__ void __launch_bounds__(CL > 1 ? 1024 : 512) kv8_select_kernel(const __grid_constant__ Kv8EvictArgs a) {
     constexpr int kSelThreads = CL > 1 ? 1024 : 512, kSelWarps = kSelThreads / 32;
@@ -411,8 +412,8 @@ LDEV uint4 ld_row(const uint8_t* p) {
 // One warp gathers kGatherBlocks destination blocks of K and V of one head: their kept rows as 16-byte pieces, all on
 // their way before the first is used (a row takes three dependent loads: the slot kept, its page, the codes), then for each
 // block the largest magnitude, the new scale, and the codes times a ratio of powers of two, in f16 (a code has at most 8
-// significant bits).  Bound by memory, each kept row read and written once: 34 us for 64 x 8 heads x 1000 rows of 64 (131 MB,
-// 3.9 TB/s: single 64-byte rows, fetched as such, do not come at the rate of whole lines).
+// significant bits).  Bound by memory, each kept row read and written once: 36 us for 64 x 8 heads x 1000 rows of 64 (131 MB,
+// 3.7 TB/s: single 64-byte rows, fetched as such, do not come at the rate of whole lines).
 constexpr int kGatherBlocks = 2;
 
 template <int FMT, int D>

@@ -104,6 +104,8 @@ struct Shape {
     static constexpr int ROWS = FEW ? 8 : 16, TILE = RW * ROWS;       // query rows of a warp and of a unit
     static constexpr int CHUNK = 4096, TOK = CHUNK / D;               // K (or V) codes and slots of a stage
     static constexpr int NB = TOK / kKv8Block, CPP = kKv8Page / TOK;  // blocks of a chunk, chunks of a page
+    // as many as shared memory holds beside the rest (two to six with RW 2: 48.2, 47.9, 47.7, 47.7 us at 8 sequences of 2048
+    // slots with 32 queries; two or three with few rows: 24.5 and 24.6 us at 64 of 1024, the same at 96 of 8192)
     static constexpr int STAGES = FEW ? 3 : RW == 1 ? 2 : 6;
     static constexpr int PART = D + 4;  // floats of one row's partial result: its sums, then M, R and l
     // items of a share: a chunk for each warp, and of groups enough that merging does not cost more than they do (one
@@ -725,10 +727,13 @@ LDEV void store_merged(const Kv8AttendArgs& a, int first, int h, int r, const fl
 // A group of RW warps walks its part of the list through its own ring of stages, each a chunk of K and of V codes and
 // their scales brought in by bulk copies; its first warp's lane 0 issues them.  With one warp a group (RW 1) the CTA takes
 // one share, its warps equal parts of it in order, and puts together at its end what they cut.
-// Few rows are bound by memory: 254 us at 96 sequences of 7192 to 8192 slots with 32 heads of 128 (1.5 GB, 6.0 TB/s), 50 us at
-// 4 of 56537 to 65537 with 24 heads of 64 (5.3 TB/s).  Many rows are bound by the instructions that widen codes for each 16
-// rows: 28 us at 8 x 32 queries over 2048 slots (100 TFLOP/s).  A list too short for the card costs 7.5 us, of which 4.5 pass
-// before the first codes arrive (lengths, then page numbers, then copies).
+// Few rows are bound by memory: 262 to 291 us by card at 96 sequences of 7192 to 8192 slots with 32 heads of 128 (1.5 GB, 5.8
+// to 5.2 TB/s), 50 us at 4 of 57,618 to 65,537 with 24 heads of 64 (248 MB, 5.0 TB/s).  Many rows are bound by the instructions
+// that widen codes for each 16 rows: 28 us at 224 queries over 8 sequences of 2048 slots (98 TFLOP/s).  A list too short for
+// the card costs 7.7 us, of which 4.5 pass before the first codes arrive (lengths, then page numbers, then copies).
+// bf16 calls: the weighted sums of a part of the list stay in the matrix unit's accumulators, which cut off what is below f32
+// (at most 2^-23 of the sum for each block of 16 slots, 2^-13 over the 664 blocks that a warp takes of 96 sequences of 8192
+// slots; the output is rounded to 2^-9).  f32 calls start a sum for each chunk and add the chunks with rounding.
 
 // what a warp of a CTA with one warp a group leaves behind
 struct Ends {
@@ -986,8 +991,8 @@ __global__ void __launch_bounds__(Shape<D, FEW, RW>::THREADS, 1) kv8_attend_kern
 }
 
 // ---- merging the shares -----------------------------------------------------------------------------------------------
-// One warp per query row and head whose unit was cut between shares, in the order of the shares.  3.3 us for a handful of rows
-// (three dependent loads), 5.6 us for 6144.
+// One warp per query row and head whose unit was cut between shares, in the order of the shares.  3.2 us for a handful of rows
+// (three dependent loads), 5.5 us for 5376.
 template <int D, bool FEW, int RW, bool F32>
 __global__ void __launch_bounds__(kThreads) kv8_merge_kernel(const __grid_constant__ Kv8AttendArgs a) {
     using SH = Shape<D, FEW, RW>;
@@ -1012,8 +1017,8 @@ __global__ void __launch_bounds__(kThreads) kv8_merge_kernel(const __grid_consta
 // ---- accumulated weights, from stored scores ------------------------------------------------------------------------------
 // With few query rows the pass over the cache also leaves its scores (4 bytes a row and slot, against d bytes of K), and
 // the weights are one elementwise pass over them: a thread takes four slots.  The kernel merges the shares too: every CTA
-// needs the merged sums of its KV head's rows, and the head's first CTA their outputs.  13 us at 4 x 65537 slots, 8 KV heads and 3
-// rows (42 MB of scores and masses), 3.7 us where there is next to nothing to do.
+// needs the merged sums of its KV head's rows, and the head's first CTA their outputs.  14 us at 4 sequences of 57,618 to 65,537
+// slots, 8 KV heads and 3 rows (39 MB of scores and masses), 3.7 us where there is next to nothing to do.
 template <int D, bool F32>
 __global__ void __launch_bounds__(128) kv8_weights_kernel(const __grid_constant__ Kv8AttendArgs a) {
     using SH = Shape<D, true, 1>;
@@ -1083,8 +1088,8 @@ __global__ void __launch_bounds__(128) kv8_weights_kernel(const __grid_constant_
 // ---- accumulated weights, from K ------------------------------------------------------------------------------------------
 // More query rows: the scores are computed again, with the finished softmax sums at hand.  The chunks of each sequence and
 // KV head are dealt to the warps of gridDim.x CTAs; a warp holds a chunk's K in registers as f16 and runs the query tiles
-// past it from shared memory.  Two CTAs an SM, with half the chunk that one would take: latency is what bounds it (14 us at 8 x 32 queries over 2048
-// slots, 96 rows a KV head).
+// past it from shared memory.  Two CTAs an SM, with half the chunk that one would take: latency is what bounds it (15 us at 224
+// queries over 8 sequences of 2048 slots, 96 rows a KV head).
 constexpr int kMassTiles = kWarps, kMassChunk = 2048;  // query tiles in shared memory, one loaded by each warp; K codes a warp holds
 
 template <int D, bool F32>
@@ -1244,6 +1249,7 @@ struct AttendLaunch {
         cudaError_t e = kv8_launch<kv8_attend_kernel<FMT, D, FEW, RW, F32>, SH::SMEM>(dim3(sm_count()), SH::THREADS, SH::SMEM, 1, s, a);
         if (e != cudaSuccess) return e;
         if (a.scores) {
+            // at most 64 CTAs a head: 16, 32, 64 and 128 take 81, 70.6, 67.5 and 67.4 us in all at 4 sequences of 65537, the same elsewhere
             const dim3 blocks(min(64, (a.kv.max_pages * kKv8Page + 511) / 512), a.kv.kv_heads, a.kv.n_seqs);
             return kv8_launch<kv8_weights_kernel<D, F32>, 0>(blocks, 128, 0, 1, s, a);
         }

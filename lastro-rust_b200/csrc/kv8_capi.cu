@@ -42,7 +42,8 @@ int check_rows(lastro_ctx* c, const lastro_rows* r, const char* what) {
     return LASTRO_OK;
 }
 
-// launches that failed: nothing was enqueued, and no object of this family holds state a failure could leave half-done
+// launches that failed: the kernels of the call before the one that failed may be enqueued, so its outputs are not to be used;
+// no object of this family holds state that it could leave half-done
 int launched(lastro_ctx* c, cudaError_t e, const char* what) {
     if (e == cudaSuccess) return LASTRO_OK;
     cudaGetLastError();
