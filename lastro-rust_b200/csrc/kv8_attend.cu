@@ -732,8 +732,9 @@ LDEV void store_merged(const Kv8AttendArgs& a, int first, int h, int r, const fl
 // that widen codes for each 16 rows: 28 us at 224 queries over 8 sequences of 2048 slots (98 TFLOP/s).  A list too short for
 // the card costs 7.7 us, of which 4.5 pass before the first codes arrive (lengths, then page numbers, then copies).
 // bf16 calls: the weighted sums of a part of the list stay in the matrix unit's accumulators, which cut off what is below f32
-// (at most 2^-23 of the sum for each block of 16 slots, 2^-13 over the 664 blocks that a warp takes of 96 sequences of 8192
-// slots; the output is rounded to 2^-9).  f32 calls start a sum for each chunk and add the chunks with rounding.
+// (at most 2^-23 of the sum for each block of 16 slots, below 2^-14 over the 311 blocks that a warp takes of 96 sequences
+// of 8192 slots with 8 KV heads of 128; the output is rounded to 2^-9).  f32 calls start a sum for each chunk and add the
+// chunks with rounding.
 
 // what a warp of a CTA with one warp a group leaves behind
 struct Ends {
